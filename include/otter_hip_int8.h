@@ -603,6 +603,96 @@ int otter_hip_upsample2d_slice_launches(int src_layout, int n, int c, int h, int
 int otter_hip_upsample2d_slice(const float* src, int src_layout, int n, int c, int h, int w, int out_h, int out_w, int mode, int align_corner,
                                int8_t* blob, int total_channels, int first_channel, float q_scale, int q_round_mode, void* stream);
 
+/* ------------------------------------------------------------------------------------------------ */
+/* transformer layers in the same numerics: symmetric int8 codes, exact int32 sums, fp32 results      */
+/* (no counterpart in the reference, which has convolutional networks only)                           */
+/* ------------------------------------------------------------------------------------------------ */
+
+/* A cache of attention keys and values in int8, in pages of OTTER_HIP_KV_BLOCK tokens of one sequence. The tokens of a page share one
+ * scale for each head and for keys and values each: a value is code * scale. The caller owns the memory, which these calls alone lay
+ * out: keys and values hold n_pages * otter_hip_kv_page_bytes(heads, head_dim) bytes each, 16-byte aligned; the scales are
+ * [n_pages][heads]. Nothing has to be cleared. head_dim 1 to 256 (the memory is that of the next multiple of 64). */
+#define OTTER_HIP_KV_BLOCK 64
+typedef struct otter_hip_kv_cache {
+    int heads, head_dim, n_pages;
+    int8_t *keys, *values;
+    float *key_scales, *value_scales;
+} otter_hip_kv_cache;
+size_t otter_hip_kv_page_bytes(int heads, int head_dim);
+
+/* Rows of several sequences, one behind the other, and where those keep their tokens. Device arrays, read by the launches (a captured
+ * call takes what they hold when it is replayed):
+ *   starts   [n_seqs + 1], not decreasing: rows starts[i] .. starts[i+1] - 1 are the LAST tokens of sequence i. Rows in front of
+ *            starts[0] and behind starts[n_seqs] belong to none: they are not read, and left as they were in results
+ *   lengths  [n_seqs]: tokens of the sequence, with those of its rows: row r of n is at position length - n + r
+ *   pages    [n_seqs][max_pages]: the page of tokens 64 b .. 64 b + 63 at [b]
+ * n_tokens: rows that the tensors have. A position below 0, behind max_pages or on a number that is no page of the pool is no token of
+ * the cache: nothing is written for it, it is read as 0, no row sees it, and a row at a position below 0 sees nothing. */
+typedef struct otter_hip_kv_batch {
+    int n_seqs, n_tokens, max_pages;
+    const int32_t *starts, *lengths, *pages;
+} otter_hip_kv_batch;
+
+/* The batch's rows into the cache. keys, values: fp32, head_dim consecutive values for each head and the heads of a row one behind the
+ * other; a row every key_stride / value_stride elements. A page's scale is s = max|x| / 127 over its tokens' finite values (0 below
+ * 2^-100), code = x / s rounded half away from zero, exactly; NaN becomes 0, an infinity +-127. Where older tokens share the page, s is
+ * no smaller than theirs was, and where it is larger their codes are rounded anew, code * s_old / s. A page that receives tokens must
+ * not be named twice in the batch; full pages, and those only read, may be shared. */
+int otter_hip_kv_append(const otter_hip_kv_cache* cache, const otter_hip_kv_batch* batch, const float* keys, size_t key_stride,
+                        const float* values, size_t value_stride, void* stream);
+
+/* The batch's rows from the cache, code * scale, [n_tokens][heads][head_dim] each; keys or values may be NULL. */
+int otter_hip_kv_read(const otter_hip_kv_cache* cache, const otter_hip_kv_batch* batch, float* keys, float* values, void* stream);
+
+/* Attention of the batch's rows over the cache, which holds their tokens already:
+ *   t_j = scale * q . k_j;  with cap: t_j = cap * tanh(t_j / cap);  with slopes: t_j -= slopes[query head] * |position - j|
+ *   out = sum_j exp(t_j) v_j / sum_j exp(t_j)
+ * over the sequence's tokens j, with causal j <= position, with window > 0 position - j < window. A row that sees none is 0; a row
+ * of q that holds a NaN or an infinity gives NaN. Query head h reads key head h / (q_heads / heads).
+ *   q    fp32, a row every q_stride elements, q_heads * head_dim consecutive values; out [n_tokens][q_heads][head_dim]
+ *   slopes  device, [q_heads], or NULL
+ * The scores are those of q rounded to 22 bits below the row's largest element, all else is fp32. A row's result does not depend on the
+ * rows of other sequences, but on how many workgroups its tokens are dealt to, which follows from n_seqs, n_tokens, max_pages and the heads.
+ * workspace: otter_hip_kv_attend_workspace_bytes (0 where one workgroup has a row's tokens), 16-byte aligned. */
+typedef struct otter_hip_kv_attend_desc {
+    int q_heads;
+    float scale;
+    float cap;  /* 0: none */
+    int causal;
+    int window; /* 0: none */
+    const float* slopes;
+} otter_hip_kv_attend_desc;
+size_t otter_hip_kv_attend_workspace_bytes(const otter_hip_kv_cache* cache, const otter_hip_kv_batch* batch, const otter_hip_kv_attend_desc* desc);
+int otter_hip_kv_attend(const otter_hip_kv_cache* cache, const otter_hip_kv_batch* batch, const otter_hip_kv_attend_desc* desc, const float* q,
+                        size_t q_stride, float* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* An int8 product for each of several experts (1: an ordinary layer) on fp32 rows that are quantized on the way in, a scale for each row:
+ *   s = max|x| / 127 over the row's finite values (0 below 2^-100), code = x / s rounded half away from zero, exactly (NaN 0, an
+ *   infinity +-127), y = act(sum_k code[k] * weight[e][n][k] * (s * scale[e][n]) + bias[e][n]), the sum exact in int32
+ * gated: the weights have 2 * out_features rows, y = silu(first half) * second half, activation_type 0. activation_type as in
+ * otter_hip_conv_desc. in_features at most 131072. weight, scale, bias (or NULL): HOST arrays [experts][rows][in_features],
+ * [experts][rows], [experts][rows]. */
+typedef struct otter_hip_linear otter_hip_linear_t;
+typedef struct {
+    int experts, in_features, out_features;
+    int gated;
+    int activation_type;
+    float activation_param0;
+} otter_hip_linear_desc;
+int otter_hip_linear_create(const otter_hip_linear_desc* desc, const int8_t* weight, const float* scale, const float* bias,
+                            otter_hip_linear_t** handle);
+int otter_hip_linear_destroy(otter_hip_linear_t* handle);
+
+/* y[r] for `rows` rows sorted by expert, [rows][out_features]. Device arrays:
+ *   x       fp32, x_rows rows of in_features values, one every x_stride elements
+ *   index   [rows]: the row of x that row r is, any number of times each (outside of x: a row of zeros), or NULL: row r itself
+ *   starts  [experts + 1], not decreasing: rows starts[e] .. starts[e+1] - 1 are expert e's; rows of none are left as they were. NULL
+ *           with one expert: all rows
+ * workspace: otter_hip_linear_workspace_bytes, 16-byte aligned. */
+size_t otter_hip_linear_workspace_bytes(const otter_hip_linear_t* handle, int x_rows, int rows);
+int otter_hip_linear_forward(const otter_hip_linear_t* handle, const float* x, size_t x_stride, int x_rows, const int32_t* index,
+                             const int32_t* starts, int rows, float* y, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -90,7 +90,10 @@ EXPORTS = ["otter_hip_init", "otter_hip_shutdown", "otter_hip_last_error", "otte
            "otter_hip_conv_dwpw_launches", "otter_hip_conv_dwpw_forward", "otter_hip_conv_maxpool_launches",
            "otter_hip_conv_forward_maxpool", "otter_hip_conv_slice_launches", "otter_hip_conv_forward_slice",
            "otter_hip_upsample2d_slice_launches", "otter_hip_upsample2d_slice",
-           "otter_hip_record_begin", "otter_hip_record_end", "otter_hip_record_launch", "otter_hip_record_destroy"]
+           "otter_hip_record_begin", "otter_hip_record_end", "otter_hip_record_launch", "otter_hip_record_destroy",
+           "otter_hip_kv_page_bytes", "otter_hip_kv_append", "otter_hip_kv_read", "otter_hip_kv_attend_workspace_bytes",
+           "otter_hip_kv_attend", "otter_hip_linear_create", "otter_hip_linear_destroy", "otter_hip_linear_workspace_bytes",
+           "otter_hip_linear_forward"]
 
 
 def load_cdll():
@@ -127,6 +130,30 @@ class End(C.Structure):
                 ("q_scale", C.c_float), ("q_round_mode", C.c_int)]
 
 
+class KvCacheArgs(C.Structure):
+    """otter_hip_kv_cache"""
+    _fields_ = [("heads", C.c_int), ("head_dim", C.c_int), ("n_pages", C.c_int), ("keys", C.c_void_p), ("values", C.c_void_p),
+                ("key_scales", C.c_void_p), ("value_scales", C.c_void_p)]
+
+
+class KvBatchArgs(C.Structure):
+    """otter_hip_kv_batch"""
+    _fields_ = [("n_seqs", C.c_int), ("n_tokens", C.c_int), ("max_pages", C.c_int), ("starts", C.c_void_p), ("lengths", C.c_void_p),
+                ("pages", C.c_void_p)]
+
+
+class KvAttendDesc(C.Structure):
+    """otter_hip_kv_attend_desc"""
+    _fields_ = [("q_heads", C.c_int), ("scale", C.c_float), ("cap", C.c_float), ("causal", C.c_int), ("window", C.c_int),
+                ("slopes", C.c_void_p)]
+
+
+class LinearDesc(C.Structure):
+    """otter_hip_linear_desc"""
+    _fields_ = [(k, C.c_int) for k in ("experts", "in_features", "out_features", "gated", "activation_type")] + \
+               [("activation_param0", C.c_float)]
+
+
 class Library:
     """The GPU library on cuda:0. Tensors are torch CUDA tensors holding the reference's packed storage."""
 
@@ -143,6 +170,9 @@ class Library:
         L.otter_hip_conv_block_layout_workspace_bytes.restype = C.c_size_t
         L.otter_hip_conv_block_form_workspace_bytes.restype = C.c_size_t
         L.otter_hip_conv_avgpool_workspace_bytes.restype = C.c_size_t
+        L.otter_hip_kv_page_bytes.restype = C.c_size_t
+        L.otter_hip_kv_attend_workspace_bytes.restype = C.c_size_t
+        L.otter_hip_linear_workspace_bytes.restype = C.c_size_t
         self.device = torch.device("cuda", device)
         self.native, self.device_index = load_binding(), device
         self._check(L.otter_hip_init(C.c_int(device)))
@@ -304,6 +334,25 @@ class Library:
 
     def conv(self, **kw):
         return Conv(self, **kw)
+
+    def kv_cache(self, n_pages, heads, head_dim):
+        return KvCache(self, n_pages, heads, head_dim)
+
+    def kv_batch(self, starts, lengths, pages, n_tokens):
+        return KvBatch(self, starts, lengths, pages, n_tokens)
+
+    def linear(self, **kw):
+        return Linear(self, **kw)
+
+    def check_tensor(self, t, dtype, shape, what, rows=False):
+        """A tensor on the library's GPU of that type and shape (None in it: any size), contiguous, with `rows` but for its first stride."""
+        if not isinstance(t, self.torch.Tensor) or t.device != self.device or t.dtype != dtype:
+            raise HipError(-2, "%s: a %s tensor on %s expected" % (what, dtype, self.device))
+        if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
+            raise HipError(-2, "%s: shape %s expected, not %s" % (what, tuple(shape), tuple(t.shape)))
+        if not (t[0] if rows and t.dim() and t.shape[0] else t).is_contiguous() or (rows and t.stride(0) < 0):
+            raise HipError(-2, "%s: not contiguous" % what)
+        return t
 
     def global_avgpool(self, x, layout, n, c, h, w):
         """otter_hip_global_avgpool: the mean over H*W of an fp32 blob, [n, c]."""
@@ -607,6 +656,120 @@ class Conv:
         if self.h:
             self.L.lib.otter_hip_conv_destroy(self.h)
             self.h = self._hp = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class KvBatch:
+    """otter_hip_kv_batch: n_tokens rows of several sequences, the last tokens of each. starts [n + 1], lengths [n] and pages
+    [n, max_pages] are int32 tensors on the GPU, which the launches read (refill them in place for a captured call)."""
+
+    def __init__(self, lib, starts, lengths, pages, n_tokens):
+        i32 = lib.torch.int32
+        lib.check_tensor(lengths, i32, (None,), "lengths")
+        n = lengths.shape[0]
+        lib.check_tensor(starts, i32, (n + 1,), "starts")
+        lib.check_tensor(pages, i32, (n, None), "pages")
+        if n_tokens < 0:
+            raise HipError(-2, "kv_batch: negative n_tokens")
+        self.starts, self.lengths, self.pages, self.n_tokens = starts, lengths, pages, int(n_tokens)
+        self.args = KvBatchArgs(n, self.n_tokens, pages.shape[1], starts.data_ptr(), lengths.data_ptr(), pages.data_ptr())
+
+
+class KvCache:
+    """otter_hip_kv_cache: n_pages pages of 64 tokens, int8 keys and values with a scale for each page and head."""
+
+    def __init__(self, lib, n_pages, heads, head_dim):
+        self.L, self.n_pages, self.heads, self.head_dim = lib, n_pages, heads, head_dim
+        page = lib.lib.otter_hip_kv_page_bytes(heads, head_dim)
+        if page == 0 or n_pages < 1:
+            raise HipError(-2, "kv_cache: heads and n_pages must be positive, head_dim 1 to 256")
+        self.keys, self.values = (lib.empty(n_pages * page, np.int8) for _ in range(2))
+        self.key_scales, self.value_scales = (lib.empty(n_pages * heads, np.float32) for _ in range(2))
+        self.args = KvCacheArgs(heads, head_dim, n_pages, *[t.data_ptr() for t in (self.keys, self.values, self.key_scales,
+                                                                                    self.value_scales)])
+
+    def append(self, batch, keys, values):
+        """otter_hip_kv_append: keys and values [n_tokens, heads, head_dim], contiguous but for the stride between rows."""
+        L, shape = self.L, (batch.n_tokens, self.heads, self.head_dim)
+        for t, what in ((keys, "keys"), (values, "values")):
+            L.check_tensor(t, L.torch.float32, shape, what, rows=True)
+        L._check(L.lib.otter_hip_kv_append(C.byref(self.args), C.byref(batch.args), L.ptr(keys), C.c_size_t(keys.stride(0)), L.ptr(values),
+                                           C.c_size_t(values.stride(0)), L.stream()))
+
+    def read(self, batch, keys=None, values=None):
+        """otter_hip_kv_read: the batch's rows as floats, [n_tokens, heads, head_dim] each. Returns (keys, values)."""
+        L, shape = self.L, (batch.n_tokens, self.heads, self.head_dim)
+        out = [L.empty(int(np.prod(shape)), np.float32).view(shape) if t is None else L.check_tensor(t, L.torch.float32, shape, "out")
+               for t in (keys, values)]
+        L._check(L.lib.otter_hip_kv_read(C.byref(self.args), C.byref(batch.args), L.ptr(out[0]), L.ptr(out[1]), L.stream()))
+        return tuple(out)
+
+    def _desc(self, q_heads, scale, cap, causal, window, slopes):
+        if slopes is not None:
+            self.L.check_tensor(slopes, self.L.torch.float32, (q_heads,), "slopes")
+        return KvAttendDesc(q_heads, self.head_dim ** -0.5 if scale is None else scale, cap, int(causal), window,
+                            None if slopes is None else slopes.data_ptr())
+
+    def attend(self, batch, q, scale=None, cap=0.0, causal=True, window=0, slopes=None, out=None, workspace=None):
+        """otter_hip_kv_attend: q [n_tokens, q_heads, head_dim], contiguous but for the stride between rows, over the cache.
+        scale None: 1 / sqrt(head_dim). Returns out, of q's shape."""
+        L, f32 = self.L, self.L.torch.float32
+        L.check_tensor(q, f32, (batch.n_tokens, None, self.head_dim), "q", rows=True)
+        desc = self._desc(q.shape[1], scale, cap, causal, window, slopes)
+        out = L.torch.empty(q.shape, dtype=f32, device=L.device) if out is None else L.check_tensor(out, f32, q.shape, "out")
+        if workspace is None:
+            need = L.lib.otter_hip_kv_attend_workspace_bytes(C.byref(self.args), C.byref(batch.args), C.byref(desc))
+            workspace = L.empty(need, np.int8) if need else None
+        L._check(L.lib.otter_hip_kv_attend(C.byref(self.args), C.byref(batch.args), C.byref(desc), L.ptr(q), C.c_size_t(q.stride(0)),
+                                           L.ptr(out), L.ptr(workspace) if workspace is not None else None,
+                                           C.c_size_t(0 if workspace is None else workspace.numel() * workspace.element_size()), L.stream()))
+        return out
+
+
+class Linear:
+    """otter_hip_linear_t: int8 weights [experts, rows, in_features] (or [rows, in_features]: one expert) with a scale for each row."""
+
+    def __init__(self, lib, *, weight, scale, bias=None, gated=False, act=0, act_p0=0.0):
+        self.L = lib
+        self.h = C.c_void_p()
+        w = np.ascontiguousarray(weight, np.int8)
+        w = w[None] if w.ndim == 2 else w
+        s, b = (None if a is None else np.ascontiguousarray(a, np.float32) for a in (scale, bias))
+        if w.ndim != 3 or s.size != w.shape[0] * w.shape[1] or (b is not None and b.size != s.size) or (gated and w.shape[1] % 2):
+            raise HipError(-2, "linear: weight [experts, rows, in_features], scale and bias [experts, rows]; an even number of rows with a gate")
+        self.experts, rows, self.in_features = w.shape
+        self.out_features = rows // 2 if gated else rows
+        d = LinearDesc(self.experts, self.in_features, self.out_features, int(gated), act, act_p0)
+        lib._check(lib.lib.otter_hip_linear_create(C.byref(d), w.ctypes.data_as(C.c_void_p), s.ctypes.data_as(C.c_void_p),
+                                                   b.ctypes.data_as(C.c_void_p) if b is not None else None, C.byref(self.h)))
+
+    def forward(self, x, starts=None, index=None, out=None, workspace=None):
+        """otter_hip_linear_forward: x [x_rows, in_features], contiguous but for the stride between rows; starts [experts + 1] and
+        index [rows] int32. Returns y [rows, out_features]."""
+        L, t = self.L, self.L.torch
+        L.check_tensor(x, t.float32, (None, self.in_features), "x", rows=True)
+        rows = x.shape[0] if index is None else L.check_tensor(index, t.int32, (None,), "index").shape[0]
+        if starts is not None:
+            L.check_tensor(starts, t.int32, (self.experts + 1,), "starts")
+        shape = (rows, self.out_features)
+        out = t.empty(shape, dtype=t.float32, device=L.device) if out is None else L.check_tensor(out, t.float32, shape, "out")
+        if workspace is None:
+            workspace = L.empty(L.lib.otter_hip_linear_workspace_bytes(self.h, x.shape[0], rows), np.int8)
+        L._check(L.lib.otter_hip_linear_forward(
+            self.h, L.ptr(x), C.c_size_t(x.stride(0)), x.shape[0], L.ptr(index) if index is not None else None,
+            L.ptr(starts) if starts is not None else None, rows, L.ptr(out), L.ptr(workspace),
+            C.c_size_t(workspace.numel() * workspace.element_size()), L.stream()))
+        return out
+
+    def close(self):
+        if self.h:
+            self.L.lib.otter_hip_linear_destroy(self.h)
+            self.h = None
 
     def __del__(self):
         try:

@@ -2,6 +2,7 @@
 // weight re-layout at create time and kernel dispatch. No kernels live here.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 #include <cstring>
 #include <mutex>
 #include <new>
@@ -11,6 +12,8 @@
 #include "common.hpp"
 #include "conv_dwpw.hpp"
 #include "conv_igemm.hpp"
+#include "kv_common.hpp"
+#include "linear.hpp"
 
 using namespace ohip;
 
@@ -2319,6 +2322,187 @@ int otter_hip_upsample2d_slice(const float* src, int src_layout, int n, int c, i
     if (launches != 1) return fail(OTTER_HIP_ERR_UNSUPPORTED, "otter_hip_upsample2d_slice: not a single launch (otter_hip_upsample2d_slice_launches)");
     OHIP_CHECK(run_upsample_slice(src, layout_pack(src_layout), blob + (size_t)first_channel * out_h * out_w, total_channels / 8, n, c, h, w, out_h, out_w, mode,
                                   align_corner ? 1 : 0, q_scale, round_half(q_round_mode), (hipStream_t)stream));
+    return OTTER_HIP_OK;
+}
+
+// -----------------------------------------------------------------------------------------------------
+// transformer layers
+// -----------------------------------------------------------------------------------------------------
+
+size_t otter_hip_kv_page_bytes(int heads, int head_dim) {
+    return heads < 1 || head_dim < 1 || head_dim > 256 ? 0 : (size_t)heads * ((head_dim + 63) / 64) * 4096;
+}
+
+// Both structs checked, and turned into what the launches take. The limits keep tiles, rows and positions in 32 bits.
+static int kv_arguments(const char* who, const otter_hip_kv_cache* cache, const otter_hip_kv_batch* batch, KvView* c, KvBatch* b) {
+    const std::string name(who);
+    if (!cache || !batch) return fail(OTTER_HIP_ERR_INVALID, name + ": null");
+    if (cache->heads < 1 || cache->head_dim < 1 || cache->n_pages < 1) return fail(OTTER_HIP_ERR_INVALID, name + ": heads, head_dim and n_pages must be positive");
+    if (cache->head_dim > 256 || cache->heads > 65536) return fail(OTTER_HIP_ERR_UNSUPPORTED, name + ": head_dim over 256 or too many heads");
+    if (!cache->keys || !cache->values || !cache->key_scales || !cache->value_scales) return fail(OTTER_HIP_ERR_INVALID, name + ": null");
+    if (((size_t)cache->keys | (size_t)cache->values) & 15) return fail(OTTER_HIP_ERR_INVALID, name + ": keys and values must be 16-byte aligned");
+    if (batch->n_seqs < 0 || batch->n_tokens < 0 || batch->max_pages < 0) return fail(OTTER_HIP_ERR_INVALID, name + ": negative size");
+    if (batch->n_seqs > (1 << 20) || batch->max_pages > (1 << 24) || (size_t)batch->n_tokens * cache->heads * cache->head_dim >= (1ull << 40) ||
+        ((size_t)batch->n_tokens / KV_BLOCK + 2 * (size_t)batch->n_seqs) * 2 * cache->heads >= (1ull << 31))
+        return fail(OTTER_HIP_ERR_UNSUPPORTED, name + ": batch too large");
+    if (batch->n_seqs > 0 && (!batch->starts || !batch->lengths || (batch->max_pages > 0 && !batch->pages)))
+        return fail(OTTER_HIP_ERR_INVALID, name + ": null");
+    *c = {cache->keys, cache->values, cache->key_scales, cache->value_scales, cache->heads, cache->head_dim, cache->n_pages, (cache->head_dim + 63) / 64};
+    *b = {batch->n_seqs, batch->n_tokens, batch->max_pages, batch->starts, batch->lengths, batch->pages};
+    return OTTER_HIP_OK;
+}
+
+int otter_hip_kv_append(const otter_hip_kv_cache* cache, const otter_hip_kv_batch* batch, const float* keys, size_t key_stride,
+                        const float* values, size_t value_stride, void* stream) {
+    KvView c;
+    KvBatch b;
+    if (int rc = kv_arguments("otter_hip_kv_append", cache, batch, &c, &b)) return rc;
+    if (b.n_seqs == 0 || b.n_tokens == 0) return OTTER_HIP_OK;
+    if (!keys || !values) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_kv_append: null");
+    OHIP_CHECK(run_kv_append(c, b, keys, key_stride, values, value_stride, (hipStream_t)stream));
+    return OTTER_HIP_OK;
+}
+
+int otter_hip_kv_read(const otter_hip_kv_cache* cache, const otter_hip_kv_batch* batch, float* keys, float* values, void* stream) {
+    KvView c;
+    KvBatch b;
+    if (int rc = kv_arguments("otter_hip_kv_read", cache, batch, &c, &b)) return rc;
+    if (b.n_seqs == 0 || b.n_tokens == 0 || (!keys && !values)) return OTTER_HIP_OK;
+    OHIP_CHECK(run_kv_read(c, b, keys, values, (hipStream_t)stream));
+    return OTTER_HIP_OK;
+}
+
+static int kv_attend_arguments(const char* who, const otter_hip_kv_cache* cache, const otter_hip_kv_batch* batch, const otter_hip_kv_attend_desc* d,
+                               KvView* c, KvBatch* b, int* splits, size_t* bytes) {
+    const std::string name(who);
+    if (int rc = kv_arguments(who, cache, batch, c, b)) return rc;
+    if (!d) return fail(OTTER_HIP_ERR_INVALID, name + ": null");
+    if (d->q_heads < 1 || d->q_heads % c->heads) return fail(OTTER_HIP_ERR_INVALID, name + ": q_heads must be a multiple of heads");
+    if (!std::isfinite(d->scale) || !std::isfinite(d->cap) || d->cap < 0 || (d->cap > 0 && !std::isfinite(d->scale / d->cap)))
+        return fail(OTTER_HIP_ERR_INVALID, name + ": scale must be finite, cap 0 or positive");
+    if (d->window < 0) return fail(OTTER_HIP_ERR_INVALID, name + ": negative window");
+    const size_t group = (size_t)(d->q_heads / c->heads), tiles = (size_t)b->n_tokens * group / 64 + b->n_seqs;
+    if ((size_t)b->n_tokens * d->q_heads >= (1ull << 31) || tiles * c->heads >= (1ull << 31)) return fail(OTTER_HIP_ERR_UNSUPPORTED, name + ": batch too large");
+    *splits = 1, *bytes = 0;
+    if (b->n_seqs == 0 || b->n_tokens == 0) return OTTER_HIP_OK;
+    *splits = kv_attend_splits((int)tiles, c->heads, b->max_pages);
+    if (*splits > 1) {
+        const size_t rows = (size_t)b->n_tokens * d->q_heads * *splits;
+        *bytes = ((2 * rows + 3) / 4 * 4 + rows * c->dim) * sizeof(float);
+    }
+    return OTTER_HIP_OK;
+}
+
+size_t otter_hip_kv_attend_workspace_bytes(const otter_hip_kv_cache* cache, const otter_hip_kv_batch* batch, const otter_hip_kv_attend_desc* desc) {
+    KvView c;
+    KvBatch b;
+    int splits;
+    size_t bytes = 0;
+    return kv_attend_arguments("otter_hip_kv_attend_workspace_bytes", cache, batch, desc, &c, &b, &splits, &bytes) ? 0 : bytes;
+}
+
+int otter_hip_kv_attend(const otter_hip_kv_cache* cache, const otter_hip_kv_batch* batch, const otter_hip_kv_attend_desc* desc, const float* q,
+                        size_t q_stride, float* out, void* workspace, size_t workspace_bytes, void* stream) {
+    KvView c;
+    KvBatch b;
+    int splits;
+    size_t bytes;
+    if (int rc = kv_attend_arguments("otter_hip_kv_attend", cache, batch, desc, &c, &b, &splits, &bytes)) return rc;
+    if (b.n_seqs == 0 || b.n_tokens == 0) return OTTER_HIP_OK;
+    if (!q || !out) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_kv_attend: null");
+    if (bytes && (!workspace || workspace_bytes < bytes)) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_kv_attend: workspace too small");
+    if (bytes && ((size_t)workspace & 15)) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_kv_attend: the workspace must be 16-byte aligned");
+    OHIP_CHECK(run_kv_attend(c, b, q, q_stride, out, desc->q_heads, desc->scale, desc->cap, desc->slopes, desc->causal, desc->window, splits,
+                             workspace, (hipStream_t)stream));
+    return OTTER_HIP_OK;
+}
+
+struct otter_hip_linear {
+    LinearView v{};
+    int8_t* w = nullptr;
+    float *scale = nullptr, *bias = nullptr;
+};
+
+int otter_hip_linear_destroy(otter_hip_linear_t* handle) {
+    if (!handle) return OTTER_HIP_OK;
+    if (handle->w) (void)hipFree(handle->w);
+    if (handle->scale) (void)hipFree(handle->scale);
+    if (handle->bias) (void)hipFree(handle->bias);
+    delete handle;
+    return OTTER_HIP_OK;
+}
+
+int otter_hip_linear_create(const otter_hip_linear_desc* desc, const int8_t* weight, const float* scale, const float* bias,
+                            otter_hip_linear_t** handle) {
+    if (handle) *handle = nullptr;
+    if (!desc || !weight || !scale || !handle) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_create: null");
+    const otter_hip_linear_desc& d = *desc;
+    if (d.experts < 1 || d.in_features < 1 || d.out_features < 1) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_create: sizes must be positive");
+    if (d.in_features > 131072) return fail(OTTER_HIP_ERR_UNSUPPORTED, "otter_hip_linear_create: the sums of more than 131072 inputs exceed 32 bits");
+    if (d.gated < 0 || d.gated > 1) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_create: gated is 0 or 1");
+    if (d.activation_type < 0 || d.activation_type > 5 || (d.gated && d.activation_type))
+        return fail(OTTER_HIP_ERR_UNSUPPORTED, "otter_hip_linear_create: activation type not supported");
+    if (d.out_features > (1 << 24) || d.experts > (1 << 16) || (size_t)d.experts * d.out_features * d.in_features >= (1ull << 40))
+        return fail(OTTER_HIP_ERR_UNSUPPORTED, "otter_hip_linear_create: weights too large");
+    const int halves = d.gated ? 2 : 1, half_tiles = (d.out_features + 15) / 16, tiles = half_tiles * halves, steps = (d.in_features + 63) / 64;
+    const size_t bytes = (size_t)d.experts * tiles * steps * 1024, rows = (size_t)d.experts * tiles * 16;
+    otter_hip_linear* h = new (std::nothrow) otter_hip_linear();
+    int8_t* const w = (int8_t*)std::calloc(bytes, 1);
+    float* const s = (float*)std::calloc(rows * 2, sizeof(float));
+    int rc = OTTER_HIP_OK;
+    if (!h || !w || !s) rc = fail(OTTER_HIP_ERR_ALLOC, "otter_hip_linear_create: host allocation failed");
+    if (rc == OTTER_HIP_OK) {
+        // tiles of 16 outputs x 64 inputs, each in the order of the matrix instruction's lanes: 16 inputs of a row are a lane's
+        for (int e = 0; e < d.experts; ++e)
+            for (int half = 0; half < halves; ++half)
+                for (int n = 0; n < d.out_features; ++n) {
+                    const size_t from = ((size_t)e * halves + half) * d.out_features + n;
+                    const size_t tile = (size_t)e * tiles + (size_t)(n / 16) * halves + half;
+                    const int8_t* const row = weight + from * d.in_features;
+                    int8_t* const to = w + tile * steps * 1024 + (size_t)(n % 16) * 16;
+                    for (int k = 0; k < d.in_features; k += 16)
+                        std::memcpy(to + (size_t)(k / 64) * 1024 + (size_t)((k / 16) % 4) * 256, row + k, (size_t)std::min(16, d.in_features - k));
+                    s[tile * 16 + n % 16] = scale[from];
+                    if (bias) s[rows + tile * 16 + n % 16] = bias[from];
+                }
+        const auto put = [&](void** dev, const void* host, size_t count) -> int {
+            OHIP_CHECK(hipMalloc(dev, count));
+            OHIP_CHECK(hipMemcpy(*dev, host, count, hipMemcpyHostToDevice));
+            return OTTER_HIP_OK;
+        };
+        rc = put((void**)&h->w, w, bytes);
+        if (rc == OTTER_HIP_OK) rc = put((void**)&h->scale, s, rows * sizeof(float));
+        if (rc == OTTER_HIP_OK && bias) rc = put((void**)&h->bias, s + rows, rows * sizeof(float));
+    }
+    std::free(w);
+    std::free(s);
+    if (rc != OTTER_HIP_OK) {
+        otter_hip_linear_destroy(h);
+        return rc;
+    }
+    h->v = {h->w, h->scale, h->bias, d.experts, d.in_features, d.out_features, tiles, steps, d.gated, d.activation_type, d.activation_param0};
+    *handle = h;
+    return OTTER_HIP_OK;
+}
+
+size_t otter_hip_linear_workspace_bytes(const otter_hip_linear_t* handle, int x_rows, int rows) {
+    return !handle || x_rows < 1 || rows < 1 ? 0 : linear_workspace_bytes(handle->v, x_rows);
+}
+
+int otter_hip_linear_forward(const otter_hip_linear_t* handle, const float* x, size_t x_stride, int x_rows, const int32_t* index,
+                             const int32_t* starts, int rows, float* y, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!handle) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_forward: null");
+    if (x_rows < 0 || rows < 0) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_forward: negative size");
+    if (!starts && handle->v.experts != 1) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_forward: several experts need starts");
+    if (!index && rows > x_rows) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_forward: more rows than x has");
+    if (rows == 0) return OTTER_HIP_OK;
+    if (!x || !y || x_rows == 0) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_forward: null");
+    if (((size_t)rows / 16 + handle->v.experts + 1) * (size_t)handle->v.tiles >= (1ull << 31))
+        return fail(OTTER_HIP_ERR_UNSUPPORTED, "otter_hip_linear_forward: too many rows");
+    if (!workspace || workspace_bytes < linear_workspace_bytes(handle->v, x_rows))
+        return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_forward: workspace too small");
+    if ((size_t)workspace & 15) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_forward: the workspace must be 16-byte aligned");
+    OHIP_CHECK(run_linear(handle->v, {x, x_stride, x_rows, index, starts, rows, y}, workspace, (hipStream_t)stream));
     return OTTER_HIP_OK;
 }
 

@@ -1,0 +1,398 @@
+// Attention over the paged int8 cache (layout: kv_common.hpp).
+//
+//   t_j = scale * q . k_j      k_j = key codes * the page's key scale        t_j = cap * tanh(t_j / cap)      t_j -= slope * |p - j|
+//   o   = sum_j exp(t_j - m) v_j / sum_j exp(t_j - m)
+//
+// Both products run on the int8 matrix cores, on the cache's bytes as they are. The float operands go in as fixed point of three
+// 8-bit digits: a query row in units of 2^-21 of its largest element's binade, the weights exp(t_j - m) in units of 2^-22 of the
+// largest weight that the row has in the page. Digit products and their sums are exact in 32 bits, so a score is off by what
+// rounding q to 22 bits makes of it, and a page's share of o by 2^-23 of the page's largest weight for each token: both are of the
+// size that sums in 32-bit floats have. (Half floats would need a second operand for the bits behind the 11th, and the bytes of
+// the cache converted for every row tile: two products at half the rate and five vector instructions for four bytes, against three
+// products at the full rate on bytes that are only loaded.)
+//
+// A wave owns 16 query rows: the tokens of a sequence times the query heads that share a key head. The scores come transposed (keys x
+// rows), so a row's statistics and scale factors live in the lanes of its column, and the weights are already where the second
+// product wants them; nothing crosses lanes but the row maxima. The running maximum and sum are fp32, one rescaling a page.
+#include "kv_common.hpp"
+
+namespace ohip {
+
+struct AttendArgs {
+    KvView c;
+    KvBatch b;
+    const float* q;
+    size_t q_stride;
+    float* out;
+    int q_heads, group;
+    float scale;  // with cap: scale / cap, else scale * log2(e)
+    float cap;    // cap * log2(e), 0: none
+    const float* slopes;
+    int causal, window;
+    int tiles, splits;
+    float *part_o, *part_ml;  // of a split: [split][row][dim], [split][row][2] with row = token * q_heads + head
+};
+
+constexpr float LOG2E = 1.44269504088896340736f;
+
+__device__ __forceinline__ float quad_max(float x) {  // over the lanes that share a column
+    x = fmaxf(x, __shfl_xor(x, 16));
+    return fmaxf(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float quad_sum(float x) {
+    x = __fadd_rn(x, __shfl_xor(x, 16));
+    return __fadd_rn(x, __shfl_xor(x, 32));
+}
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// tanh of scores that are at most a few thousand: 1 - 2 / (exp(2 x) + 1) loses the bits of a small x, where the series goes on to x^9
+// (|x| < 1/4: the next term is below 2^-27 x).
+__device__ __forceinline__ float tanh_of(float x) {
+    const float a = __builtin_fabsf(x), y = __fmul_rn(x, x);
+    const float big = __fmaf_rn(-2.f, __fdividef(1.f, __fadd_rn(fast_exp2(__fmul_rn(a, 2.f * LOG2E)), 1.f)), 1.f);
+    float s = __fmaf_rn(y, 62.f / 2835.f, -17.f / 315.f);
+    s = __fmaf_rn(y, s, 2.f / 15.f);
+    s = __fmaf_rn(y, s, -1.f / 3.f);
+    s = __fmaf_rn(__fmul_rn(y, a), s, a);
+    return __builtin_copysignf(a < 0.25f ? s : big, x);
+}
+
+// Three signed digits of four fixed-point numbers (u = number + 0x8080 in the low 24 bits): u's low two bytes less 128, and the third.
+__device__ __forceinline__ void split_digits(const unsigned (&u)[4], int& low, int& mid, int& high) {
+    const unsigned ab = __builtin_amdgcn_perm(u[1], u[0], 0x05010400);  // a0 b0 a1 b1
+    const unsigned cd = __builtin_amdgcn_perm(u[3], u[2], 0x05010400);
+    low = (int)(__builtin_amdgcn_perm(cd, ab, 0x05040100) ^ 0x80808080u);
+    mid = (int)(__builtin_amdgcn_perm(cd, ab, 0x07060302) ^ 0x80808080u);
+    const unsigned a2b2 = __builtin_amdgcn_perm(u[1], u[0], 0x0c0c0602), c2d2 = __builtin_amdgcn_perm(u[3], u[2], 0x0c0c0602);
+    high = (int)__builtin_amdgcn_perm(c2d2, a2b2, 0x05040100);
+}
+
+typedef ohip_v4i v4i;
+__device__ __forceinline__ v4i mma(v4i a, v4i b, v4i c) { return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0); }
+// (high * 256 + mid) * 256 + low: the first step is below 2^31 for 256 dims
+__device__ __forceinline__ float join_digits(int high, int mid, int low) { return __fmaf_rn((float)((high << 8) + mid), 256.f, (float)low); }
+
+template <int KC>
+struct Queries {
+    v4i digit[3][KC];  // high, mid, low
+    float unit;        // what 1 stands for (NaN: the row holds a NaN or an infinity)
+};
+
+// A lane's share of its row: 16 dims of every 64.
+template <int KC>
+__device__ __forceinline__ void load_queries(Queries<KC>& q, const float* __restrict__ row, int dim, bool whole) {
+    const int g = (int)(threadIdx.x >> 4) & 3;
+    float x[KC][16];
+    float most = 0.f;
+    bool odd = false;
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+        const int d0 = c * 64 + g * 16;
+        if (whole) {  // (rows at 16 bytes, whole quads)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                float4 f = {0.f, 0.f, 0.f, 0.f};
+                if (d0 + e < dim) f = *reinterpret_cast<const float4*>(row + d0 + e);
+                x[c][e] = f.x, x[c][e + 1] = f.y, x[c][e + 2] = f.z, x[c][e + 3] = f.w;
+            }
+        } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) x[c][e] = d0 + e < dim ? row[d0 + e] : 0.f;
+        }
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const float a = __builtin_fabsf(x[c][e]);
+            odd |= !(a < __builtin_inff());
+            most = fmaxf(most, a);
+        }
+    }
+    most = quad_max(odd ? __builtin_inff() : most);
+    odd = !(most < __builtin_inff());
+    // units of 2^(e - 21), most in [2^e, 2^(e + 1)): at most 2^22 of them. (A row below 2^-100 counts as 0.)
+    const int e = (int)(__float_as_uint(most) >> 23) - 127;
+    const bool none = odd || e < -100;
+    const float per = none ? 0.f : __uint_as_float((unsigned)(127 + 21 - e) << 23);
+    q.unit = odd ? __builtin_nanf("") : none ? 0.f : __uint_as_float((unsigned)(127 - 21 + e) << 23);
+#pragma unroll
+    for (int c = 0; c < KC; ++c)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            unsigned u[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                u[r] = (unsigned)((none ? 0 : (int)__builtin_rintf(__fmul_rn(x[c][4 * t + r], per))) + 0x8080);
+            }
+            int lo, mi, hi;
+            split_digits(u, lo, mi, hi);
+            q.digit[2][c][t] = lo, q.digit[1][c][t] = mi, q.digit[0][c][t] = hi;
+        }
+}
+
+template <int KC>
+struct Running {
+    float o[4 * KC][4];  // [16 dims][lane group's four]
+    float m, l;          // maximum (log2), this lane's share of the sum
+};
+
+// One page into a wave's 16 rows. kp, vp: the page's head in lane order (the lane's own 16 bytes of a tile). lo, hi: positions of the
+// page that this lane's row sees, [lo, hi); whole: all 64, for every row. away: position of the row less that of the page.
+template <int KC, bool EXTRA>
+__device__ __forceinline__ void attend_page(Running<KC>& s, const Queries<KC>& q, const int8_t* kp, const int8_t* vp, float factor, float v_scale,
+                                            float cap, float slope, int lo, int hi, int away, bool whole) {
+    const int g = (int)(threadIdx.x >> 4) & 3;
+    float t[4][4];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+        v4i a[3] = {};
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            const v4i k = *reinterpret_cast<const v4i*>(kp + (c * 4 + kt) * 1024);
+#pragma unroll
+            for (int n = 0; n < 3; ++n) a[n] = mma(k, q.digit[n][c], a[n]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float x = __fmul_rn(join_digits(a[0][r], a[1][r], a[2][r]), factor);
+            if constexpr (EXTRA) {
+                if (cap != 0.f) x = __fmul_rn(tanh_of(x), cap);
+                x = __fmaf_rn(-slope, __builtin_fabsf((float)(away - (16 * kt + 4 * g + r))), x);
+            }
+            t[kt][r] = x;
+        }
+    }
+    if (!whole) {
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int j = 16 * kt + 4 * g + r;
+                if (j < lo || j >= hi) t[kt][r] = -__builtin_inff();
+            }
+    }
+    float most = t[0][0];
+#pragma unroll
+    for (int i = 1; i < 16; ++i) most = fmaxf(most, t[i >> 2][i & 3]);
+    most = quad_max(most);
+    const bool sees = most != -__builtin_inff();
+    const float base = sees ? most : 0.f;
+    float sum = 0.f;
+    v4i w[3];
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) {
+        unsigned u[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float e = fast_exp2(__fadd_rn(t[kt][r], -base));
+            sum = __fadd_rn(sum, e);
+            u[r] = __float_as_uint(__fmaf_rn(e, 0x1p22f, 8388608.f + 32896.f));  // 2^23 + 0x8080: the mantissa is the rounded number
+        }
+        int low, mid, high;
+        split_digits(u, low, mid, high);
+        w[2][kt] = low, w[1][kt] = mid, w[0][kt] = high;
+    }
+    const float m = fmaxf(s.m, most);
+    const float keep = s.m == -__builtin_inff() ? 0.f : fast_exp2(__fadd_rn(s.m, -m));
+    const float take = sees ? fast_exp2(__fadd_rn(most, -m)) : 0.f;
+    s.m = m;
+    s.l = __fmaf_rn(s.l, keep, __fmul_rn(sum, take));
+    const float put = __fmul_rn(__fmul_rn(take, 0x1p-22f), v_scale);
+#pragma unroll
+    for (int dt = 0; dt < 4 * KC; ++dt) {
+        const v4i v = *reinterpret_cast<const v4i*>(vp + dt * 1024);
+        v4i a[3];
+#pragma unroll
+        for (int n = 0; n < 3; ++n) a[n] = mma(v, w[n], v4i{0, 0, 0, 0});
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s.o[dt][r] = __fmaf_rn(join_digits(a[0][r], a[1][r], a[2][r]), put, __fmul_rn(s.o[dt][r], keep));
+    }
+}
+
+// 64 rows a workgroup, one key head: each wave a tile of 16 of them, or, where a sequence has at most 32, 16 rows of which two or
+// four waves share the pages out between them and join what they have in LDS.
+template <int KC, bool EXTRA>
+__global__ void __launch_bounds__(256) kv_attend_kernel(AttendArgs a) {
+    __shared__ __attribute__((aligned(16))) float joined[4][16][64 * KC + 4];
+    __shared__ float joined_ml[4][16][2];
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), g = lane >> 4;
+    const int head = (int)(blockIdx.x % (unsigned)a.c.heads);
+    const int tile = a.tiles - 1 - (int)(blockIdx.x / (unsigned)a.c.heads);  // (a causal prompt's last tiles have the most to read)
+    const int i = kv_find(a.b.starts, a.b.n_seqs, a.b.n_tokens, a.group, 64, 1, tile);
+    const KvSeq s = kv_sequence(a.b, i);
+    const int row0 = (tile - kv_tile_base(a.b.starts, i, a.b.n_tokens, a.group, 64, 1)) * 64, rows = s.count * a.group;
+    if (row0 < 0 || row0 >= rows) return;
+    const int tiles = (min(rows - row0, 64) + 15) >> 4;            // of 16 rows
+    const int shares = tiles == 1 ? 4 : tiles == 2 ? 2 : 1;        // waves that share a tile's pages
+    const int mine = wave / shares, share = wave % shares;         // (a fourth wave of three tiles has none: it joins the barriers)
+    const bool works = mine < tiles;
+    const int r = row0 + mine * 16 + (lane & 15);
+    const int row = min(r, rows - 1), token = row / a.group, q_head = head * a.group + row % a.group;
+    const int p = s.first + token;
+    const size_t out_row = (size_t)(s.begin + token) * a.q_heads + q_head;
+    // positions that this row sees: [lo, hi)
+    const int stored = min(s.length, a.b.max_pages * KV_BLOCK);
+    const int hi = p < 0 ? 0 : a.causal ? min(stored, p + 1) : stored;
+    const int lo = a.window > 0 && p >= a.window ? p - a.window + 1 : 0;
+
+    Running<KC> run;
+    run.m = -__builtin_inff(), run.l = 0.f;
+#pragma unroll
+    for (int dt = 0; dt < 4 * KC; ++dt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) run.o[dt][e] = 0.f;
+    if (works) {
+        // what the wave's rows see: rows are in the order of their tokens
+        const int first_hi = __builtin_amdgcn_readlane(hi, 0), last_hi = __builtin_amdgcn_readlane(hi, 15);
+        const int first_lo = __builtin_amdgcn_readlane(lo, 0), last_lo = __builtin_amdgcn_readlane(lo, 15);
+        const int page0 = first_lo / KV_BLOCK, pages = max((last_hi + KV_BLOCK - 1) / KV_BLOCK - page0, 0);
+        const int parts = a.splits * shares, part = (int)blockIdx.y * shares + share;
+        const int each = (pages + parts - 1) / parts;
+        const int from = page0 + min(part * each, pages), to = page0 + min((part + 1) * each, pages);
+        if (from < to) {
+            Queries<KC> q;
+            const bool whole_rows = a.c.dim % 4 == 0 && a.q_stride % 4 == 0 && ((size_t)a.q & 15) == 0;
+            load_queries<KC>(q, a.q + (size_t)(s.begin + token) * a.q_stride + (size_t)q_head * a.c.dim, a.c.dim, whole_rows);
+            const float factor = __fmul_rn(q.unit, a.scale);
+            float slope = 0.f;
+            if constexpr (EXTRA) slope = a.slopes ? __fmul_rn(a.slopes[q_head], LOG2E) : 0.f;
+            const int32_t* const table = a.b.pages + (size_t)i * a.b.max_pages;
+            int ids = 0;
+            for (int pg = from; pg < to; ++pg) {
+                if (((pg - from) & 63) == 0) ids = table[min(pg + lane, to - 1)];
+                const int id = __builtin_amdgcn_readlane(ids, (pg - from) & 63);
+                if ((unsigned)id >= (unsigned)a.c.n_pages) continue;  // not a page: its tokens are not seen
+                const size_t at = a.c.at(id, head);
+                const size_t sc = (size_t)id * a.c.heads + head;
+                const int base = pg * KV_BLOCK;
+                const bool whole = base + KV_BLOCK <= first_hi && base >= last_lo;
+                attend_page<KC, EXTRA>(run, q, a.c.k + at + lane * 16, a.c.v + at + lane * 16, __fmul_rn(factor, a.c.ks[sc]), a.c.vs[sc], a.cap,
+                                       slope, lo - base, hi - base, p - base, whole);
+            }
+        }
+        run.l = quad_sum(run.l);
+    }
+    if (shares > 1) {
+        if (works) {
+#pragma unroll
+            for (int dt = 0; dt < 4 * KC; ++dt)
+                *reinterpret_cast<float4*>(&joined[wave][lane & 15][dt * 16 + g * 4]) = {run.o[dt][0], run.o[dt][1], run.o[dt][2], run.o[dt][3]};
+            if (g == 0) joined_ml[wave][lane & 15][0] = run.m, joined_ml[wave][lane & 15][1] = run.l;
+        }
+        __syncthreads();
+        if (!works || share != 0) return;
+        float m = run.m;
+        for (int n = 1; n < shares; ++n) m = fmaxf(m, joined_ml[wave + n][lane & 15][0]);
+        float keep = run.m == -__builtin_inff() ? 0.f : fast_exp2(__fadd_rn(run.m, -m));
+        run.l = __fmul_rn(run.l, keep);
+#pragma unroll
+        for (int dt = 0; dt < 4 * KC; ++dt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) run.o[dt][e] = __fmul_rn(run.o[dt][e], keep);
+        for (int n = 1; n < shares; ++n) {
+            const float mn = joined_ml[wave + n][lane & 15][0];
+            keep = mn == -__builtin_inff() ? 0.f : fast_exp2(__fadd_rn(mn, -m));
+            run.l = __fmaf_rn(joined_ml[wave + n][lane & 15][1], keep, run.l);
+#pragma unroll
+            for (int dt = 0; dt < 4 * KC; ++dt) {
+                const float4 f = *reinterpret_cast<const float4*>(&joined[wave + n][lane & 15][dt * 16 + g * 4]);
+                run.o[dt][0] = __fmaf_rn(f.x, keep, run.o[dt][0]), run.o[dt][1] = __fmaf_rn(f.y, keep, run.o[dt][1]);
+                run.o[dt][2] = __fmaf_rn(f.z, keep, run.o[dt][2]), run.o[dt][3] = __fmaf_rn(f.w, keep, run.o[dt][3]);
+            }
+        }
+        run.m = m;
+    }
+    if (!works || r >= rows) return;
+    float* to = a.out;
+    size_t at = out_row;
+    float by = run.l == 0.f ? 0.f : __fdiv_rn(1.f, run.l);  // (a row that sees nothing is 0)
+    if (a.splits > 1) {
+        at = (size_t)blockIdx.y * ((size_t)a.b.n_tokens * a.q_heads) + out_row;
+        to = a.part_o;
+        by = 1.f;
+        if (g == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * at) = {run.m, run.l};
+        if (run.l == 0.f) return;  // (kv_join_kernel reads no sums of an empty share)
+    }
+    to += at * a.c.dim;
+    const bool quads = a.c.dim % 4 == 0 && ((size_t)to & 15) == 0;
+#pragma unroll
+    for (int dt = 0; dt < 4 * KC; ++dt) {
+        const int d = dt * 16 + g * 4;
+        if (quads) {
+            if (d < a.c.dim)
+                *reinterpret_cast<float4*>(to + d) = {__fmul_rn(run.o[dt][0], by), __fmul_rn(run.o[dt][1], by), __fmul_rn(run.o[dt][2], by),
+                                                      __fmul_rn(run.o[dt][3], by)};
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (d + e < a.c.dim) to[d + e] = __fmul_rn(run.o[dt][e], by);
+        }
+    }
+}
+
+// The splits of a row joined: a wave for each (token, query head).
+__global__ void __launch_bounds__(256) kv_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, float* __restrict__ out,
+                                                      const int32_t* __restrict__ starts, int n_seqs, int n_rows, int q_heads, int dim, int splits) {
+    const int row = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
+    if (row >= n_rows) return;
+    const int token = row / q_heads;
+    if (token < starts[0] || token >= starts[n_seqs]) return;  // rows of no sequence stay as they were
+    float m = -__builtin_inff();
+    for (int n = 0; n < splits; ++n) m = fmaxf(m, part_ml[2 * ((size_t)n * n_rows + row)]);
+    float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < splits; ++n) {
+        const size_t at = (size_t)n * n_rows + row;
+        const float ln = part_ml[2 * at + 1], mn = part_ml[2 * at];
+        if (ln == 0.f) continue;
+        const float keep = mn == -__builtin_inff() ? 1.f : fast_exp2(__fadd_rn(mn, -m));  // (NaN weights have no maximum)
+        l = __fmaf_rn(ln, keep, l);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (lane + 64 * e < dim) o[e] = __fmaf_rn(part_o[at * dim + lane + 64 * e], keep, o[e]);
+    }
+    const float by = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        if (lane + 64 * e < dim) out[(size_t)row * dim + lane + 64 * e] = __fmul_rn(o[e], by);
+}
+
+// Shares that the pages of a tile are cut into, each a workgroup's. A wave reads 16 KB of a page of 128 dims at a time and two
+// workgroups of four fill a compute unit's memory pipe, so there are to be 512 workgroups where the pages give each wave two.
+int kv_attend_splits(int tiles, int heads, int max_pages) {
+    const int have = tiles * heads;
+    const int want = (512 + have - 1) / have, most = max_pages / 8;
+    return want < most ? (want < 1 ? 1 : want) : (most < 1 ? 1 : most);
+}
+int kv_attend_tiles(int n_tokens, int n_seqs, int group) { return (int)((size_t)n_tokens * group / 64) + n_seqs; }
+
+template <int KC>
+static void launch_attend(const AttendArgs& a, bool extra, dim3 grid, hipStream_t stream) {
+    if (extra) launch(kv_attend_kernel<KC, true>, grid, dim3(256), 0, stream, a);
+    else launch(kv_attend_kernel<KC, false>, grid, dim3(256), 0, stream, a);
+}
+
+hipError_t run_kv_attend(const KvView& c, const KvBatch& b, const float* q, size_t q_stride, float* out, int q_heads, float scale, float cap,
+                         const float* slopes, int causal, int window, int splits, void* workspace, hipStream_t stream) {
+    AttendArgs a;
+    a.c = c, a.b = b, a.q = q, a.q_stride = q_stride, a.out = out, a.q_heads = q_heads, a.group = q_heads / c.heads;
+    a.scale = cap != 0.f ? scale / cap : scale * LOG2E;
+    a.cap = cap * LOG2E;
+    a.slopes = slopes, a.causal = causal, a.window = window;
+    a.tiles = kv_attend_tiles(b.n_tokens, b.n_seqs, a.group), a.splits = splits;
+    const size_t rows = (size_t)b.n_tokens * q_heads;
+    a.part_ml = (float*)workspace;
+    a.part_o = a.part_ml + (splits > 1 ? (2 * rows * splits + 3) / 4 * 4 : 0);
+    const dim3 grid((unsigned)a.tiles * (unsigned)c.heads, (unsigned)splits);
+    const bool extra = cap != 0.f || slopes != nullptr;
+    switch (c.chunks) {
+    case 1: launch_attend<1>(a, extra, grid, stream); break;
+    case 2: launch_attend<2>(a, extra, grid, stream); break;
+    case 3: launch_attend<3>(a, extra, grid, stream); break;
+    default: launch_attend<4>(a, extra, grid, stream); break;
+    }
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || splits == 1) return e;
+    launch(kv_join_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, (const float*)a.part_o, (const float*)a.part_ml, out, b.starts,
+           b.n_seqs, (int)rows, q_heads, c.dim, splits);
+    return hipGetLastError();
+}
+
+}  // namespace ohip

@@ -1,0 +1,106 @@
+// What the launches on the paged int8 cache of keys and values share: its layout, the batch's geometry and the rounding to codes.
+#pragma once
+
+#include "common.hpp"
+
+namespace ohip {
+
+constexpr int KV_BLOCK = 64;  // tokens of a page: they share a scale for each head
+
+// Scales below this count as 0: their codes are all 0. It keeps the exact comparisons of code_of clear of the smallest numbers.
+constexpr float KV_LEAST_SCALE = 0x1p-100f;
+
+// A page of one head is 4 * chunks tiles of 1 KiB for the keys and as many for the values, chunks = ceil(head_dim / 64), each the
+// operand of one 16x16x64 matrix instruction in lane order: a lane's 16 bytes at 16 * lane.
+//   keys   tile [dims / 64][tokens / 16], row = token % 16, contraction = dim % 64
+//   values tile [dims / 16], row = dim % 16, contraction = token, in the order that the scores' lanes hold the tokens:
+//          slot 16 g + 4 t + r is token 16 t + 4 g + r, so that the weights of a row go into the second product without leaving
+//          their lanes
+// Both are loaded as whole contiguous KiB. Dims behind head_dim are 0.
+struct KvView {
+    int8_t *k, *v;
+    float *ks, *vs;  // [pages][heads]
+    int heads, dim, n_pages, chunks;
+    __host__ __device__ size_t head_bytes() const { return (size_t)chunks * 4096; }
+    __device__ size_t at(int page, int head) const { return ((size_t)page * heads + head) * head_bytes(); }
+};
+// byte of (token, dim) in a page's head
+__host__ __device__ inline int kv_key_byte(int token, int dim) {
+    return ((dim >> 6) * 4 + (token >> 4)) * 1024 + ((dim >> 4) & 3) * 256 + (token & 15) * 16 + (dim & 15);
+}
+__host__ __device__ inline int kv_value_byte(int token, int dim) {
+    return (dim >> 4) * 1024 + ((token >> 2) & 3) * 256 + (dim & 15) * 16 + (token >> 4) * 4 + (token & 3);
+}
+
+struct KvBatch {
+    int n_seqs, n_tokens, max_pages;
+    const int32_t *starts, *lengths, *pages;
+};
+
+// One sequence of a batch as the kernels see it: what a table that is wrong could say is cut to what the buffers hold.
+struct KvSeq {
+    int begin, count;  // its rows
+    int length;        // tokens, with those of the rows
+    int first;         // position of its first row (below 0: the batch says more rows than tokens)
+};
+__device__ __forceinline__ KvSeq kv_sequence(const KvBatch& b, int i) {
+    KvSeq s;
+    s.begin = min(max(b.starts[i], 0), b.n_tokens);
+    s.count = min(max(b.starts[i + 1], s.begin), b.n_tokens) - s.begin;
+    s.length = max(b.lengths[i], 0);
+    s.first = s.length - s.count;
+    return s;
+}
+
+// Work is dealt to tiles of `unit` rows of a sequence without a list of them: sequence i's tiles begin at starts[i] * mul / unit +
+// slack * i, which leaves each at least as many as it needs (ceil(n / unit) <= floor difference + 1, and one more where a tile is
+// aligned to positions, not to rows). The largest i whose tiles begin at or before `tile`, by the lanes of a wave: a load for each 64-fold.
+__device__ __forceinline__ int kv_tile_base(const int32_t* starts, int i, int limit, int mul, int unit, int slack) {
+    return (int)((unsigned)(min(max(starts[i], 0), limit) * mul) / (unsigned)unit) + slack * i;
+}
+__device__ __forceinline__ int kv_find(const int32_t* starts, int n, int limit, int mul, int unit, int slack, int tile) {
+    const int lane = (int)(threadIdx.x & 63);
+    int lo = 0;
+    while (n > 1) {
+        const int step = (n + 63) >> 6, i = lane * step;
+        const bool before = i < n && kv_tile_base(starts, lo + min(i, n - 1), limit, mul, unit, slack) <= tile;
+        const int k = max(__popcll(__ballot(before)), 1) - 1;
+        lo += k * step;
+        n = min(step, n - k * step);
+    }
+    return __builtin_amdgcn_readfirstlane(lo);
+}
+
+// |x| of a finite value, 0 for an infinity or NaN: what a scale is found from.
+__device__ __forceinline__ float finite_size(float x) {
+    const float a = __builtin_fabsf(x);
+    return a < __builtin_inff() ? a : 0.f;
+}
+__device__ __forceinline__ float scale_of(float most) {
+    const float s = __fdiv_rn(most, 127.f);
+    return s < KV_LEAST_SCALE ? 0.f : s;
+}
+
+// x / s rounded half away from zero, at most 127, exactly (NaN: 0). The product with the rounded reciprocal is off by less than
+// 2^-15, so its rounding is off by one at most; whether it is tells the sign of |x| - (c -+ 1/2) s, which one fused multiply-add
+// has right. s is at least KV_LEAST_SCALE (then no result of it underflows), inv = 1 / s.
+__device__ __forceinline__ int code_of(float x, float s, float inv) {
+    const float a = fminf(__builtin_fabsf(x), __fmul_rn(s, 128.f));  // (an infinity; NaN becomes 128 steps: taken out below)
+    float c = __builtin_floorf(__fadd_rn(__fmul_rn(a, inv), 0.5f));
+    if (__fmaf_rn(__fadd_rn(c, -0.5f), -s, a) < 0.f) c = __fadd_rn(c, -1.f);
+    else if (__fmaf_rn(__fadd_rn(c, 0.5f), -s, a) >= 0.f) c = __fadd_rn(c, 1.f);
+    const int i = min((int)c, 127);
+    return x == x ? (x < 0.f ? -i : i) : 0;
+}
+
+// kv_cache.hip
+hipError_t run_kv_append(const KvView& c, const KvBatch& b, const float* k, size_t k_stride, const float* v, size_t v_stride, hipStream_t stream);
+hipError_t run_kv_read(const KvView& c, const KvBatch& b, float* k, float* v, hipStream_t stream);
+
+// kv_attend.hip
+int kv_attend_tiles(int n_tokens, int n_seqs, int group);
+int kv_attend_splits(int tiles, int heads, int max_pages);
+hipError_t run_kv_attend(const KvView& c, const KvBatch& b, const float* q, size_t q_stride, float* out, int q_heads, float scale, float cap,
+                         const float* slopes, int causal, int window, int splits, void* workspace, hipStream_t stream);
+
+}  // namespace ohip
