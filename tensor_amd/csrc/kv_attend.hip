@@ -328,30 +328,64 @@ __global__ void __launch_bounds__(256) kv_attend_kernel(AttendArgs a) {
     }
 }
 
-// The splits of a row joined: a wave for each (token, query head).
+// The splits of a row joined: a workgroup for each (token, query head), a quarter of the splits for each of its waves, whose sums meet
+// in LDS. A wave walks its splits a few at a time, so that their loads are in flight together: one by one, by a single wave, 128 splits
+// of 28 rows took 110 us, three times the attention itself.
 __global__ void __launch_bounds__(256) kv_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, float* __restrict__ out,
                                                       const int32_t* __restrict__ starts, int n_seqs, int n_rows, int q_heads, int dim, int splits) {
-    const int row = (int)blockIdx.x * 4 + ((int)threadIdx.x >> 6), lane = (int)threadIdx.x & 63;
-    if (row >= n_rows) return;
+    __shared__ float sums[4][256];
+    __shared__ float share_of[4][2];
+    const int row = (int)blockIdx.x, lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const int token = row / q_heads;
     if (token < starts[0] || token >= starts[n_seqs]) return;  // rows of no sequence stay as they were
+    const int each = (splits + 3) / 4, from = min(wave * each, splits), to = min(from + each, splits);
+    // the wave's largest maximum; NaN weights have none: -infinity and a sum that is not 0
     float m = -__builtin_inff();
-    for (int n = 0; n < splits; ++n) m = fmaxf(m, part_ml[2 * ((size_t)n * n_rows + row)]);
+    for (int n = from + lane; n < to; n += 64) m = fmaxf(m, part_ml[2 * ((size_t)n * n_rows + row)]);
+#pragma unroll
+    for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
     float l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int n = 0; n < splits; ++n) {
-        const size_t at = (size_t)n * n_rows + row;
-        const float ln = part_ml[2 * at + 1], mn = part_ml[2 * at];
-        if (ln == 0.f) continue;
-        const float keep = mn == -__builtin_inff() ? 1.f : fast_exp2(__fadd_rn(mn, -m));  // (NaN weights have no maximum)
+    for (int n0 = from; n0 < to; n0 += 64) {
+        // a split for each lane: its weight
+        float keep = 0.f, ln = 0.f;
+        if (n0 + lane < to) {
+            const float2 ml = *reinterpret_cast<const float2*>(part_ml + 2 * ((size_t)(n0 + lane) * n_rows + row));
+            ln = ml.y;
+            if (ln != 0.f) keep = ml.x == -__builtin_inff() ? 1.f : fast_exp2(__fadd_rn(ml.x, -m));
+        }
+        const int count = min(to - n0, 64);
         l = __fmaf_rn(ln, keep, l);
+        for (int n = 0; n < count; n += 8) {
+            float k[8], f[8][4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (lane + 64 * e < dim) o[e] = __fmaf_rn(part_o[at * dim + lane + 64 * e], keep, o[e]);
+            for (int i = 0; i < 8; ++i) {
+                k[i] = n + i < count ? __shfl(keep, n + i) : 0.f;  // (of an empty split 0 too: its sums are not written)
+                const float* const at = part_o + ((size_t)(n0 + min(n + i, count - 1)) * n_rows + row) * dim;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f[i][e] = lane + 64 * e < dim ? at[lane + 64 * e] : 0.f;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) o[e] = k[i] != 0.f ? __fmaf_rn(f[i][e], k[i], o[e]) : o[e];
+        }
     }
-    const float by = l == 0.f ? 0.f : __fdiv_rn(1.f, l);
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        if (lane + 64 * e < dim) out[(size_t)row * dim + lane + 64 * e] = __fmul_rn(o[e], by);
+    for (int k = 32; k; k >>= 1) l = __fadd_rn(l, __shfl_xor(l, k));
+#pragma unroll
+    for (int e = 0; e < 4; ++e) sums[wave][lane + 64 * e] = o[e];
+    if (lane == 0) share_of[wave][0] = m, share_of[wave][1] = l;
+    __syncthreads();
+    m = fmaxf(fmaxf(share_of[0][0], share_of[1][0]), fmaxf(share_of[2][0], share_of[3][0]));
+    float total = 0.f, sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float lw = share_of[w][1], mw = share_of[w][0];
+        const float keep = lw == 0.f ? 0.f : mw == -__builtin_inff() ? 1.f : fast_exp2(__fadd_rn(mw, -m));
+        total = __fmaf_rn(lw, keep, total);
+        sum = __fmaf_rn(sums[w][threadIdx.x], keep, sum);
+    }
+    if ((int)threadIdx.x < dim) out[(size_t)row * dim + threadIdx.x] = total == 0.f ? 0.f : __fdiv_rn(sum, total);
 }
 
 // Shares that the pages of a tile are cut into, each a workgroup's. A wave reads 16 KB of a page of 128 dims at a time and two
@@ -390,7 +424,7 @@ hipError_t run_kv_attend(const KvView& c, const KvBatch& b, const float* q, size
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || splits == 1) return e;
-    launch(kv_join_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, (const float*)a.part_o, (const float*)a.part_ml, out, b.starts,
+    launch(kv_join_kernel, dim3((unsigned)rows), dim3(256), 0, stream, (const float*)a.part_o, (const float*)a.part_ml, out, b.starts,
            b.n_seqs, (int)rows, q_heads, c.dim, splits);
     return hipGetLastError();
 }

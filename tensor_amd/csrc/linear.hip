@@ -22,14 +22,42 @@ static LinearCodes linear_codes(const LinearView& w, int x_rows, void* workspace
 }
 size_t linear_workspace_bytes(const LinearView& w, int x_rows) { return ((size_t)x_rows * 4 + 255) / 256 * 256 + (size_t)x_rows * w.steps * 64; }
 
-// A workgroup a row: its largest size, then its codes (the row is in the cache by then).
+// Four inputs of a row from d on; those behind its last are 0.
+__device__ __forceinline__ float4 row_quad(const float* __restrict__ row, int d, int in, bool quads) {
+    float4 f = {0.f, 0.f, 0.f, 0.f};
+    if (quads) {
+        if (d < in) f = *reinterpret_cast<const float4*>(row + d);
+    } else {
+        if (d < in) f.x = row[d];
+        if (d + 1 < in) f.y = row[d + 1];
+        if (d + 2 < in) f.z = row[d + 2];
+        if (d + 3 < in) f.w = row[d + 3];
+    }
+    return f;
+}
+__device__ __forceinline__ int codes_of_quad(const float4& f, float s, float inv) {
+    if (!(s > 0.f)) return 0;
+    return (code_of(f.x, s, inv) & 0xff) | ((code_of(f.y, s, inv) & 0xff) << 8) | ((code_of(f.z, s, inv) & 0xff) << 16) | (code_of(f.w, s, inv) << 24);
+}
+__device__ __forceinline__ float most_of_quad(const float4& f) {
+    return fmaxf(fmaxf(finite_size(f.x), finite_size(f.y)), fmaxf(finite_size(f.z), finite_size(f.w)));
+}
+
+// A workgroup a row: its largest size, then its codes. 4096 inputs stay in registers, what is behind them is read again.
 __global__ void __launch_bounds__(256) linear_codes_kernel(const float* __restrict__ x, size_t stride, int in, int padded, float* __restrict__ scale,
                                                            int8_t* __restrict__ codes) {
+    constexpr int KEPT = 4;
     __shared__ float most_of[4];
     const int tid = (int)threadIdx.x;
     const float* const row = x + (size_t)blockIdx.x * stride;
+    const bool quads = in % 4 == 0 && stride % 4 == 0 && ((size_t)x & 15) == 0;
+    float4 kept[KEPT];
+#pragma unroll
+    for (int u = 0; u < KEPT; ++u) kept[u] = row_quad(row, 4 * tid + 1024 * u, in, quads);
     float most = 0.f;
-    for (int d = tid; d < in; d += 256) most = fmaxf(most, finite_size(row[d]));
+#pragma unroll
+    for (int u = 0; u < KEPT; ++u) most = fmaxf(most, most_of_quad(kept[u]));
+    for (int d = 4 * tid + 1024 * KEPT; d < in; d += 1024) most = fmaxf(most, most_of_quad(row_quad(row, d, in, quads)));
 #pragma unroll
     for (int m = 32; m; m >>= 1) most = fmaxf(most, __shfl_xor(most, m));
     if ((tid & 63) == 0) most_of[tid >> 6] = most;
@@ -38,15 +66,10 @@ __global__ void __launch_bounds__(256) linear_codes_kernel(const float* __restri
     const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
     if (tid == 0) scale[blockIdx.x] = s;
     int* const to = reinterpret_cast<int*>(codes + (size_t)blockIdx.x * padded);
-    for (int d = 4 * tid; d < padded; d += 1024) {
-        unsigned v = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const int c = d + e < in && s > 0.f ? code_of(row[d + e], s, inv) : 0;
-            v |= (unsigned)(c & 0xff) << (8 * e);
-        }
-        to[d >> 2] = (int)v;
-    }
+    for (int u = 0; u < KEPT; ++u)
+        if (4 * tid + 1024 * u < padded) to[tid + 256 * u] = codes_of_quad(kept[u], s, inv);
+    for (int d = 4 * tid + 1024 * KEPT; d < padded; d += 1024) to[d >> 2] = codes_of_quad(row_quad(row, d, in, quads), s, inv);
 }
 
 struct LinearArgs {
