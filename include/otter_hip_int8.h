@@ -692,6 +692,9 @@ int otter_hip_linear_destroy(otter_hip_linear_t* handle);
 size_t otter_hip_linear_workspace_bytes(const otter_hip_linear_t* handle, int x_rows, int rows);
 int otter_hip_linear_forward(const otter_hip_linear_t* handle, const float* x, size_t x_stride, int x_rows, const int32_t* index,
                              const int32_t* starts, int rows, float* y, void* workspace, size_t workspace_bytes, void* stream);
+/* For tests and profiling: which launch otter_hip_linear_forward takes for that many rows: 0 the one for few rows, 1 to 3 those for many,
+ * 32 x 64, 64 x 64 and 64 x 128 results a wave. The results are the same, bit for bit. */
+int otter_hip_linear_kernel_kind(const otter_hip_linear_t* handle, int rows);
 
 #ifdef __cplusplus
 }

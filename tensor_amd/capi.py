@@ -93,7 +93,7 @@ EXPORTS = ["otter_hip_init", "otter_hip_shutdown", "otter_hip_last_error", "otte
            "otter_hip_record_begin", "otter_hip_record_end", "otter_hip_record_launch", "otter_hip_record_destroy",
            "otter_hip_kv_page_bytes", "otter_hip_kv_append", "otter_hip_kv_read", "otter_hip_kv_attend_workspace_bytes",
            "otter_hip_kv_attend", "otter_hip_linear_create", "otter_hip_linear_destroy", "otter_hip_linear_workspace_bytes",
-           "otter_hip_linear_forward"]
+           "otter_hip_linear_forward", "otter_hip_linear_kernel_kind"]
 
 
 def load_cdll():
@@ -747,6 +747,12 @@ class Linear:
         d = LinearDesc(self.experts, self.in_features, self.out_features, int(gated), act, act_p0)
         lib._check(lib.lib.otter_hip_linear_create(C.byref(d), w.ctypes.data_as(C.c_void_p), s.ctypes.data_as(C.c_void_p),
                                                    b.ctypes.data_as(C.c_void_p) if b is not None else None, C.byref(self.h)))
+
+    def kernel_kind(self, rows):
+        """otter_hip_linear_kernel_kind: 0 the launch for few rows, 1 to 3 those for many."""
+        r = self.L.lib.otter_hip_linear_kernel_kind(self.h, rows)
+        self.L._check(min(r, 0))
+        return r
 
     def forward(self, x, starts=None, index=None, out=None, workspace=None):
         """otter_hip_linear_forward: x [x_rows, in_features], contiguous but for the stride between rows; starts [experts + 1] and

@@ -2489,6 +2489,11 @@ size_t otter_hip_linear_workspace_bytes(const otter_hip_linear_t* handle, int x_
     return !handle || x_rows < 1 || rows < 1 ? 0 : linear_workspace_bytes(handle->v, x_rows);
 }
 
+int otter_hip_linear_kernel_kind(const otter_hip_linear_t* handle, int rows) {
+    if (!handle || rows < 1) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_kernel_kind: null or no rows");
+    return linear_choice(handle->v, rows);
+}
+
 int otter_hip_linear_forward(const otter_hip_linear_t* handle, const float* x, size_t x_stride, int x_rows, const int32_t* index,
                              const int32_t* starts, int rows, float* y, void* workspace, size_t workspace_bytes, void* stream) {
     if (!handle) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_forward: null");

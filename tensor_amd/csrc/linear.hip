@@ -12,7 +12,7 @@ typedef ohip_v4i v4i;
 
 struct LinearCodes {
     float* scale;   // [x_rows]
-    int8_t* codes;  // [x_rows][steps * 64]
+    int8_t* codes;  // [x_rows][whole pairs of steps]
 };
 static LinearCodes linear_codes(const LinearView& w, int x_rows, void* workspace) {
     LinearCodes c;
@@ -20,7 +20,9 @@ static LinearCodes linear_codes(const LinearView& w, int x_rows, void* workspace
     c.codes = (int8_t*)workspace + ((size_t)x_rows * 4 + 255) / 256 * 256;
     return c;
 }
-size_t linear_workspace_bytes(const LinearView& w, int x_rows) { return ((size_t)x_rows * 4 + 255) / 256 * 256 + (size_t)x_rows * w.steps * 64; }
+// bytes of a row of codes: whole pairs of steps, zeros behind the last input
+__host__ __device__ inline size_t linear_row_bytes(int steps) { return (size_t)(steps + 1) / 2 * 128; }
+size_t linear_workspace_bytes(const LinearView& w, int x_rows) { return ((size_t)x_rows * 4 + 255) / 256 * 256 + (size_t)x_rows * linear_row_bytes(w.steps); }
 
 // Four inputs of a row from d on; those behind its last are 0.
 __device__ __forceinline__ float4 row_quad(const float* __restrict__ row, int d, int in, bool quads) {
@@ -108,98 +110,250 @@ __device__ __forceinline__ int linear_source(const LinearArgs& a, int row) {
     return (unsigned)i < (unsigned)a.x_rows ? i : -1;
 }
 
-// Four consecutive outputs of one row.
-template <bool GATED>
-__device__ __forceinline__ void linear_store(const LinearArgs& a, int expert, int n_tile, int row, float xs, const v4i& acc, const v4i& acc_up) {
-    const int g = (int)(threadIdx.x >> 4) & 3;
-    const size_t at = ((size_t)expert * a.w.tiles + (size_t)n_tile * (GATED ? 2 : 1)) * 16 + g * 4;
-    float v[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float b = a.w.bias ? a.w.bias[at + e] : 0.f;
-        v[e] = __fmaf_rn((float)acc[e], __fmul_rn(xs, a.w.scale[at + e]), b);
-        if constexpr (GATED) {
-            const float bu = a.w.bias ? a.w.bias[at + 16 + e] : 0.f;
-            const float up = __fmaf_rn((float)acc_up[e], __fmul_rn(xs, a.w.scale[at + 16 + e]), bu);
-            v[e] = __fmul_rn(__fdiv_rn(v[e], __fadd_rn(1.f, __expf(-v[e]))), up);
-        } else v[e] = activate(v[e], a.w.act, a.w.act_p0);
-    }
-    const int n = n_tile * 16 + g * 4;
-    float* const to = a.y + (size_t)row * a.w.out + n;
+// What the epilogue needs of four consecutive outputs: a lane's share of an output tile.
+struct LinearOut {
+    float4 scale, bias;
+};
+__device__ __forceinline__ LinearOut linear_out(const LinearArgs& a, int expert, int tile) {
+    const size_t at = ((size_t)expert * a.w.tiles + tile) * 16 + ((threadIdx.x >> 4) & 3) * 4;
+    LinearOut o;
+    o.scale = *reinterpret_cast<const float4*>(a.w.scale + at);
+    o.bias = {0.f, 0.f, 0.f, 0.f};
+    if (a.w.bias) o.bias = *reinterpret_cast<const float4*>(a.w.bias + at);
+    return o;
+}
+__device__ __forceinline__ float4 linear_value(const v4i& acc, float xs, const LinearOut& o) {
+    return {__fmaf_rn((float)acc[0], __fmul_rn(xs, o.scale.x), o.bias.x), __fmaf_rn((float)acc[1], __fmul_rn(xs, o.scale.y), o.bias.y),
+            __fmaf_rn((float)acc[2], __fmul_rn(xs, o.scale.z), o.bias.z), __fmaf_rn((float)acc[3], __fmul_rn(xs, o.scale.w), o.bias.w)};
+}
+__device__ __forceinline__ float gate(float g, float up) { return __fmul_rn(__fdiv_rn(g, __fadd_rn(1.f, __expf(-g))), up); }
+// Four consecutive outputs of one row, `column` the first.
+__device__ __forceinline__ void linear_put(const LinearArgs& a, int row, int column, const float4& v) {
+    float* const to = a.y + (size_t)row * a.w.out + column;
     if (a.w.out % 4 == 0 && ((size_t)a.y & 15) == 0) {
-        if (n < a.w.out) *reinterpret_cast<float4*>(to) = {v[0], v[1], v[2], v[3]};
+        if (column < a.w.out) *reinterpret_cast<float4*>(to) = v;
     } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (n + e < a.w.out) to[e] = v[e];
+        if (column < a.w.out) to[0] = v.x;
+        if (column + 1 < a.w.out) to[1] = v.y;
+        if (column + 2 < a.w.out) to[2] = v.z;
+        if (column + 3 < a.w.out) to[3] = v.w;
     }
 }
+template <bool GATED>
+__device__ __forceinline__ void linear_store(const LinearArgs& a, int row, float xs, int n_tile, const v4i& acc, const v4i& acc_up, const LinearOut& o,
+                                             const LinearOut& o_up) {
+    float4 v = linear_value(acc, xs, o);
+    if constexpr (GATED) {
+        const float4 u = linear_value(acc_up, xs, o_up);
+        v = {gate(v.x, u.x), gate(v.y, u.y), gate(v.z, u.z), gate(v.w, u.w)};
+    } else if (a.w.act) {
+        v = {activate(v.x, a.w.act, a.w.act_p0), activate(v.y, a.w.act, a.w.act_p0), activate(v.z, a.w.act, a.w.act_p0), activate(v.w, a.w.act, a.w.act_p0)};
+    }
+    linear_put(a, row, n_tile * 16 + (int)((threadIdx.x >> 4) & 3) * 4, v);
+}
 
-// 16 outputs (gated: 16 of either half) x 16 RT rows a workgroup, the inputs dealt to its four waves, whose sums meet in LDS. Both
-// operands come straight from memory in lane order; this is the launch for few rows, where reading the weights is the work.
-template <int RT, bool GATED>
-__global__ void __launch_bounds__(256) linear_few_kernel(LinearArgs a) {
-    constexpr int G = GATED ? 2 : 1;
-    __shared__ v4i sums[4][G * RT][64];
+// 16 outputs (gated: 16 of either half) x 16 rows a workgroup, the inputs dealt to its W waves, whose sums meet in LDS. Both operands
+// come straight from memory in lane order, several steps of them asked for before the first is used; this is the launch for few rows,
+// where reading the weights is the work. (32 and 64 rows a workgroup, which read the weights less often, were the fastest of all launches
+// for no size.)
+template <bool GATED, int W>
+__global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
+    constexpr int G = GATED ? 2 : 1, AHEAD = 4;
+    __shared__ v4i sums[W][G][64];
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const unsigned n_tiles = (unsigned)a.w.tiles / G;
     const int n_tile = (int)(blockIdx.x % n_tiles);
-    const LinearTile t = linear_tile(a, (int)(blockIdx.x / n_tiles), 16 * RT);
+    const LinearTile t = linear_tile(a, (int)(blockIdx.x / n_tiles), 16);
     if (t.begin >= t.end) return;
-    const size_t step_bytes = (size_t)a.w.steps * 64;
-    const int8_t* const w = a.w.w + ((size_t)t.expert * a.w.tiles + (size_t)n_tile * G) * a.w.steps * 1024 + lane * 16;
-    const int8_t* x[RT];
+    const int steps = a.w.steps;
+    const int8_t* const w = a.w.w + ((size_t)t.expert * a.w.tiles + (size_t)n_tile * G) * steps * 1024;
+    const unsigned lane16 = (unsigned)lane * 16u;
+    const int row = t.begin + (lane & 15), src = linear_source(a, min(row, t.end - 1));
+    const int8_t* const x = a.codes + (size_t)max(src, 0) * linear_row_bytes(steps) + (lane >> 4) * 16;
+    v4i acc[G] = {};
+    const int each = (steps + W - 1) / W, to = min((wave + 1) * each, steps);
+    for (int s = wave * each; s < to; s += AHEAD) {
+        v4i k[AHEAD][G], b[AHEAD];
 #pragma unroll
-    for (int i = 0; i < RT; ++i) {
-        const int src = linear_source(a, min(t.begin + i * 16 + (lane & 15), t.end - 1));
-        x[i] = a.codes + (size_t)max(src, 0) * step_bytes + (lane >> 4) * 16;
-    }
-    v4i acc[G][RT] = {};
-    for (int s = wave; s < a.w.steps; s += 4) {
-        v4i b[RT];
+        for (int u = 0; u < AHEAD; ++u) {
+            const int at = min(s + u, to - 1);
 #pragma unroll
-        for (int i = 0; i < RT; ++i) b[i] = *reinterpret_cast<const v4i*>(x[i] + s * 64);
+            for (int h = 0; h < G; ++h) k[u][h] = *reinterpret_cast<const v4i*>(w + ((size_t)h * steps + at) * 1024 + lane16);
+            b[u] = *reinterpret_cast<const v4i*>(x + (size_t)at * 64);
+        }
 #pragma unroll
-        for (int h = 0; h < G; ++h) {
-            const v4i k = *reinterpret_cast<const v4i*>(w + ((size_t)h * a.w.steps + s) * 1024);
+        for (int u = 0; u < AHEAD; ++u) {
+            if (s + u >= to) break;
 #pragma unroll
-            for (int i = 0; i < RT; ++i) acc[h][i] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k, b[i], acc[h][i], 0, 0, 0);
+            for (int h = 0; h < G; ++h) acc[h] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][h], b[u], acc[h], 0, 0, 0);
         }
     }
 #pragma unroll
-    for (int h = 0; h < G; ++h)
-#pragma unroll
-        for (int i = 0; i < RT; ++i) sums[wave][h * RT + i][lane] = acc[h][i];
+    for (int h = 0; h < G; ++h) sums[wave][h][lane] = acc[h];
     __syncthreads();
-    if (wave >= RT) return;
+    if (wave != 0 || row >= t.end) return;
     v4i sum[2] = {};
 #pragma unroll
     for (int h = 0; h < G; ++h)
 #pragma unroll
-        for (int n = 0; n < 4; ++n) sum[h] += sums[n][h * RT + wave][lane];
-    const int row = t.begin + wave * 16 + (lane & 15);
-    if (row >= t.end) return;
-    const int src = linear_source(a, row);
-    linear_store<GATED>(a, t.expert, n_tile, row, src < 0 ? 0.f : a.scale[src], sum[0], sum[1]);
+        for (int n = 0; n < W; ++n) sum[h] += sums[n][h][lane];
+    const LinearOut o = linear_out(a, t.expert, n_tile * G), o_up = linear_out(a, t.expert, n_tile * G + G - 1);
+    linear_store<GATED>(a, row, src < 0 ? 0.f : a.scale[src], n_tile, sum[0], sum[1], o, o_up);
 }
 
-template <int RT>
+// 64 NT outputs x 16 RT rows a workgroup, 16 NT outputs a wave: the launch for many rows. A wave loads its weights, which no other
+// wave of the workgroup reads, straight into registers, a stage of 128 inputs ahead; the rows' codes, which all four waves read, go
+// through LDS, in lane order too (a 16-byte piece of a row is a lane's). A stage is 8 NT RT matrix instructions a wave against 2 RT KB
+// from LDS and 2 NT KB from memory: with 4 and 8 that is 64 and 32 bytes a cycle of a compute unit's 128 and 64.
+template <int NT, int RT, bool GATED>
+__global__ void __launch_bounds__(256, 2) linear_many_kernel(LinearArgs a) {
+    constexpr int MINE = RT / 4;  // tiles of 16 rows that a wave brings in
+    __shared__ v4i rows[3][RT][2][64];
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const unsigned n_blocks = (unsigned)(a.w.tiles + 4 * NT - 1) / (4 * NT);
+    const LinearTile t = linear_tile(a, (int)(blockIdx.x / n_blocks), 16 * RT);
+    if (t.begin >= t.end) return;
+    const int tile0 = ((int)(blockIdx.x % n_blocks) * 4 + wave) * NT, steps = a.w.steps;
+    const size_t row_bytes = linear_row_bytes(steps);
+    const int8_t* w[NT];  // (the same for every lane: the lane's share is a 32-bit offset to it)
+#pragma unroll
+    for (int n = 0; n < NT; ++n) w[n] = a.w.w + ((size_t)t.expert * a.w.tiles + min(tile0 + n, a.w.tiles - 1)) * steps * 1024;
+    const unsigned lane16 = (unsigned)lane * 16u;
+    const int8_t* x[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; ++i) {
+        const int src = linear_source(a, min(t.begin + (wave * MINE + i) * 16 + (lane & 15), t.end - 1));
+        x[i] = a.codes + (size_t)max(src, 0) * row_bytes + (lane >> 4) * 16;
+    }
+    // (steps go in twos: an odd count ends on a step of zeros of the rows)
+    const int even = (steps + 1) & ~1;
+    const auto load_w = [&](v4i (&to)[NT], int s) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) to[n] = *reinterpret_cast<const v4i*>(w[n] + (size_t)min(s, steps - 1) * 1024 + lane16);
+    };
+    v4i xr[MINE][2];
+    const auto load_x = [&](int s) {
+#pragma unroll
+        for (int i = 0; i < MINE; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) xr[i][h] = *reinterpret_cast<const v4i*>(x[i] + (size_t)min(s, even - 2) * 64 + h * 64);
+    };
+    const auto put_x = [&](int slot) {
+#pragma unroll
+        for (int i = 0; i < MINE; ++i)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) rows[slot][wave * MINE + i][h][lane] = xr[i][h];
+    };
+    v4i acc[NT][RT] = {};
+    v4i wr[4][NT];
+    load_x(0);
+    put_x(0);
+    load_x(2);
+#pragma unroll
+    for (int s = 0; s < 4; ++s) load_w(wr[s], s);
+    put_x(1);
+    load_x(4);
+    int slot = 0;
+    // A stage: two steps. Weights are asked for four steps before their use, rows two stages before it, one before they go to LDS. No
+    // branch in the loop: behind one the compiler waits for every load in flight.
+    const auto stage = [&](auto parity, int s) {
+        constexpr int P = decltype(parity)::value;
+        // this stage's rows are in LDS, and nobody reads the slot before it any more (loads from memory stay in flight)
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        const v4i* const from = &rows[slot][0][0][lane];
+        v4i b[3];
+        b[0] = from[0], b[1] = from[128];
+#pragma unroll
+        for (int i = 0; i < 2 * RT; ++i) {  // (row tile, step): a tile is read from LDS two tiles before its products
+            const int h = i / RT, r = i % RT;
+            if (i + 2 < 2 * RT) b[(i + 2) % 3] = from[((i + 2) % RT * 2 + (i + 2) / RT) * 64];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) acc[n][r] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wr[2 * P + h][n], b[i % 3], acc[n][r], 0, 0, 0);
+            if (r == RT - 1) load_w(wr[2 * P + h], s + h + 4);
+            if (i == RT - 1) {
+                put_x(slot == 0 ? 2 : slot - 1);
+                load_x(s + 6);
+            }
+            __builtin_amdgcn_sched_barrier(0);  // (left alone the compiler reads a tile right in front of its products)
+        }
+        slot = slot == 2 ? 0 : slot + 1;
+    };
+    int s = 0;
+    for (; s + 4 <= even; s += 4) {
+        stage(std::integral_constant<int, 0>{}, s);
+        stage(std::integral_constant<int, 1>{}, s + 2);
+    }
+    if (s < even) stage(std::integral_constant<int, 0>{}, s);
+    constexpr int G = GATED ? 2 : 1;
+#pragma unroll
+    for (int n = 0; n < NT; n += G) {
+        if (tile0 + n >= a.w.tiles) break;
+        const LinearOut o = linear_out(a, t.expert, tile0 + n), o_up = linear_out(a, t.expert, tile0 + n + G - 1);
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+            const int row = t.begin + r * 16 + (lane & 15);
+            if (row >= t.end) continue;
+            const int src = linear_source(a, row);
+            linear_store<GATED>(a, row, src < 0 ? 0.f : a.scale[src], (tile0 + n) / G, acc[n][r], acc[n + G - 1][r], o, o_up);
+        }
+    }
+}
+
+template <int W>
 static void launch_few(const LinearArgs& a, const LinearRows& r, hipStream_t stream) {
-    const dim3 grid((unsigned)(a.w.tiles / (a.w.gated ? 2 : 1)) * (unsigned)linear_row_tiles(a.w, r, 16 * RT));
-    if (a.w.gated) launch(linear_few_kernel<RT, true>, grid, dim3(256), 0, stream, a);
-    else launch(linear_few_kernel<RT, false>, grid, dim3(256), 0, stream, a);
+    const dim3 grid((unsigned)(a.w.tiles / (a.w.gated ? 2 : 1)) * (unsigned)linear_row_tiles(a.w, r, 16));
+    if (a.w.gated) launch(linear_few_kernel<true, W>, grid, dim3(64 * W), 0, stream, a);
+    else launch(linear_few_kernel<false, W>, grid, dim3(64 * W), 0, stream, a);
+}
+
+template <int NT, int RT>
+static void launch_many(const LinearArgs& a, const LinearRows& r, hipStream_t stream) {
+    const dim3 grid((unsigned)((a.w.tiles + 4 * NT - 1) / (4 * NT)) * (unsigned)linear_row_tiles(a.w, r, 16 * RT));
+    if (a.w.gated) launch(linear_many_kernel<NT, RT, true>, grid, dim3(256), 0, stream, a);
+    else launch(linear_many_kernel<NT, RT, false>, grid, dim3(256), 0, stream, a);
+}
+
+// The launch that is the fastest by a model of the measured ones (3 to 128 steps of inputs, 512 to 8192 outputs, 1 to 16384 rows, 1 to
+// 64 experts; microseconds without the codes). The one for few rows reads weights and rows from the caches at 10 TB/s, 16 x 16 results
+// at a time, but waits 1.2 for every four steps of a wave. The others take `each` for a stage of a workgroup by itself and `busy` where
+// every compute unit has one, n times that for n: 64 x 64 results a wave are the least traffic, 32 x 64 start the soonest. Against
+// the fastest of the five: 4096 x 4096 weights, 128 rows 23.1 us (few: 26.1), 512 rows 27.3 (64 x 64 a wave: 35.0), 2048 rows 61.9 (32
+// x 64: 73.7), 8192 rows 196 (64 x 64: 214).
+int linear_choice(const LinearView& w, int rows) {
+    const auto row_tiles = [&](int unit) {
+        return w.experts == 1 ? (rows + unit - 1) / unit : rows / unit + (rows < w.experts ? rows : w.experts) * 0.5;
+    };
+    const double stages = (w.steps + 1) / 2, weights = (double)w.tiles * w.steps * 1024;
+    const auto many = [&](int nt, int rt, double start, double each, double busy) {
+        const double load = (w.tiles + 4 * nt - 1) / (4 * nt) * row_tiles(16 * rt) / 256 * busy;
+        return start + stages * (load > each ? load : each);
+    };
+    const double waits = ((w.steps + 31) / 32) * 1.2, reads = row_tiles(16) * 2 * weights / 10e6;
+    const double t[4] = {2.5 + (waits > reads ? waits : reads), many(2, 4, 5, 0.5, 0.48), many(4, 4, 7, 0.8, 0.69), many(4, 8, 9, 1.65, 1.2)};
+    int best = 0;
+    for (int i = 1; i < 4; ++i)
+        if (t[i] < t[best]) best = i;
+    return best;
 }
 
 hipError_t run_linear(const LinearView& w, const LinearRows& r, void* workspace, hipStream_t stream) {
     const LinearCodes c = linear_codes(w, r.x_rows, workspace);
-    if (r.x_rows) launch(linear_codes_kernel, dim3((unsigned)r.x_rows), dim3(256), 0, stream, r.x, r.x_stride, w.in, w.steps * 64, c.scale, c.codes);
-    hipError_t e = hipGetLastError();
+    launch(linear_codes_kernel, dim3((unsigned)r.x_rows), dim3(256), 0, stream, r.x, r.x_stride, w.in, (int)linear_row_bytes(w.steps), c.scale, c.codes);
+    const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     const LinearArgs a{w, c.scale, c.codes, r.index, r.starts, r.x_rows, r.rows, r.y};
-    // rows of a tile: few where an expert has few (the tiles of an expert without rows end at once)
-    if (r.rows <= 16 * w.experts) launch_few<1>(a, r, stream);
-    else if (r.rows <= 32 * w.experts) launch_few<2>(a, r, stream);
-    else launch_few<4>(a, r, stream);
+    switch (linear_choice(w, r.rows)) {
+    case 0: {
+        // eight waves share the inputs where the workgroups alone would leave compute units without work
+        const double groups = (double)(w.tiles / (w.gated ? 2 : 1)) * ((r.rows + 15) / 16);
+        if (groups < 1024 && w.steps >= 16) launch_few<8>(a, r, stream);
+        else launch_few<4>(a, r, stream);
+        break;
+    }
+    case 1: launch_many<2, 4>(a, r, stream); break;
+    case 2: launch_many<4, 4>(a, r, stream); break;
+    default: launch_many<4, 8>(a, r, stream); break;
+    }
     return hipGetLastError();
 }
 

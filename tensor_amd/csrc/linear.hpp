@@ -22,6 +22,7 @@ struct LinearRows {
     float* y;
 };
 size_t linear_workspace_bytes(const LinearView& w, int x_rows);
+int linear_choice(const LinearView& w, int rows);  // otter_hip_linear_kernel_kind
 hipError_t run_linear(const LinearView& w, const LinearRows& r, void* workspace, hipStream_t stream);
 
 }  // namespace ohip

@@ -130,6 +130,38 @@ def test_a_row_is_the_same_whatever_stands_beside_it(hip):
         assert hip.torch.equal(whole[a:e], layer.forward(x[a:e]))
 
 
+@pytest.mark.parametrize("kind,experts,k,n,rows,gated", [
+    (1, 1, 1000, 1030, 1500, False), (1, 5, 260, 501, 3000, False), (1, 4, 448, 640, 900, True), (1, 3, 64, 520, 16000, False),
+    (2, 1, 1000, 1030, 9000, False), (2, 3, 320, 1900, 9001, False), (2, 2, 130, 1500, 9000, True), (2, 1, 64, 4200, 9000, False),
+    (3, 1, 1090, 4100, 4100, False), (3, 2, 576, 3900, 5000, False), (3, 3, 500, 1990, 6000, True), (3, 1, 64, 8200, 16000, False)])
+def test_launches_for_many_rows(hip, kind, experts, k, n, rows, gated):
+    """Every row of each of the launches for many rows, against the launch for few rows, 16 at a time of one expert, bit for bit; that
+    one is compared with the model above, and here at the first and the last of its rows."""
+    torch = hip.torch
+    rng = np.random.default_rng(kind * rows)
+    w, s, b = weights(rng, experts, 2 * n if gated else n, k)
+    layer = hip.linear(weight=w, scale=s, bias=b, gated=gated)
+    assert layer.kernel_kind(rows) == kind and layer.kernel_kind(16) == 0
+    cuts = np.sort(rng.integers(0, rows + 1, experts - 1))
+    starts = np.concatenate([[3], np.maximum(cuts, 3), [rows]]).astype(np.int32)
+    x = hip.to_device(rng.normal(0, 1, (rows // 2, k)).astype(np.float32))
+    index = rng.integers(0, rows // 2, rows).astype(np.int32)
+    out = layer.forward(x, dev(hip, starts), dev(hip, index), out=torch.full((rows, n), 5.0, device=hip.device))
+    assert (out[:3] == 5).all()
+    for e in range(experts):
+        one = hip.linear(weight=w[e], scale=s[e], bias=b[e], gated=gated)
+        for a in [*range(int(starts[e]), int(starts[e + 1]), 16)]:
+            z = min(a + 16, int(starts[e + 1]))
+            i = dev(hip, index[a:z])
+            assert torch.equal(out[a:z], one.forward(x, index=i)), (e, a)
+        one.close()
+    for r in (3, rows - 1):
+        e = int(np.searchsorted(starts, r, side="right")) - 1
+        xn = x[int(index[r])].cpu().numpy()[None]
+        check_close(out[r:r + 1].cpu().numpy(), *linear(xn, w[e:e + 1], s[e:e + 1], b[e:e + 1], np.zeros((1, n), np.float32), gated=gated))
+    layer.close()
+
+
 def test_a_transformer_layer_replayed(hip):
     """The operators as a layer uses them -- projection, append, attention, projection, experts with a gate, the product behind it --
     eagerly on a stream of its own, then captured and replayed on new inputs."""
