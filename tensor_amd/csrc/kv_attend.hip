@@ -35,13 +35,19 @@ struct AttendArgs {
 
 constexpr float LOG2E = 1.44269504088896340736f;
 
-__device__ __forceinline__ float quad_max(float x) {  // over the lanes that share a column
-    x = fmaxf(x, __shfl_xor(x, 16));
-    return fmaxf(x, __shfl_xor(x, 32));
+// Over the four lanes that share a column, 16 apart. (The exchanges put both halves, or both rows of 16, of a register beside each
+// other in two; no LDS.)
+__device__ __forceinline__ float quad_max(float x) {
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float quad_sum(float x) {
-    x = __fadd_rn(x, __shfl_xor(x, 16));
-    return __fadd_rn(x, __shfl_xor(x, 32));
+    auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __fadd_rn(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __fadd_rn(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
@@ -134,104 +140,200 @@ struct Running {
     float m, l;          // maximum (log2), this lane's share of the sum
 };
 
-// One page into a wave's 16 rows. kp, vp: the page's head in lane order (the lane's own 16 bytes of a tile). lo, hi: positions of the
-// page that this lane's row sees, [lo, hi); whole: all 64, for every row. away: position of the row less that of the page.
-template <int KC, bool EXTRA>
-__device__ __forceinline__ void attend_page(Running<KC>& s, const Queries<KC>& q, const int8_t* kp, const int8_t* vp, float factor, float v_scale,
-                                            float cap, float slope, int lo, int hi, int away, bool whole) {
+// What a step of NP pages has beside their codes: the scales, and the positions of their first tokens.
+template <int NP>
+struct Pages {
+    float k_scale[NP], v_scale[NP];
+    int first[NP];
+    bool all;  // all of them are pages of the pool
+};
+// What a lane's row sees, [lo, hi), and where it is itself.
+struct RowView {
+    int lo, hi, p;
+    float slope;
+};
+
+// NP pages into a wave's 16 rows. key(page, tile) and value(page, tile): the lane's 16 bytes of a tile; keys_done and values_done: called
+// when the last of them is used. whole: every row sees all of them. Two pages at a time share the conversions of the second product's sums and the rescaling of o, a quarter of the vector
+// instructions of one: the weights go in as multiples of the pages' value scales, in units of 2^-22 of the largest such product.
+template <int KC, int EXTRA, int NP, typename Key, typename Value, typename KeysDone, typename ValuesDone>
+__device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& q, const Key& key, const Value& value, const KeysDone& keys_done,
+                                             const ValuesDone& values_done, const Pages<NP>& at, float factor, float cap, const RowView& row,
+                                             bool whole) {
     const int g = (int)(threadIdx.x >> 4) & 3;
-    float t[4][4];
+    float t[NP][4][4], most_of[NP];
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-        v4i a[3] = {};
+    for (int p = 0; p < NP; ++p) {
+        const float unit = __fmul_rn(factor, at.k_scale[p]);  // of the page's scores, log2
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            const v4i k = *reinterpret_cast<const v4i*>(kp + (c * 4 + kt) * 1024);
+        for (int kt = 0; kt < 4; ++kt) {
+            v4i a[3] = {};
 #pragma unroll
-            for (int n = 0; n < 3; ++n) a[n] = mma(k, q.digit[n][c], a[n]);
-        }
+            for (int c = 0; c < KC; ++c) {
+                const v4i k = key(p, c * 4 + kt);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            float x = __fmul_rn(join_digits(a[0][r], a[1][r], a[2][r]), factor);
-            if constexpr (EXTRA) {
-                if (cap != 0.f) x = __fmul_rn(tanh_of(x), cap);
-                x = __fmaf_rn(-slope, __builtin_fabsf((float)(away - (16 * kt + 4 * g + r))), x);
+                for (int n = 0; n < 3; ++n) a[n] = mma(k, q.digit[n][c], a[n]);
             }
-            t[kt][r] = x;
-        }
-    }
-    if (!whole) {
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int j = 16 * kt + 4 * g + r;
-                if (j < lo || j >= hi) t[kt][r] = -__builtin_inff();
+                float x = __fmul_rn(join_digits(a[0][r], a[1][r], a[2][r]), unit);
+                if constexpr (EXTRA != 0) {
+                    if (EXTRA == 1 || cap != 0.f) x = __fmul_rn(tanh_of(x), cap);
+                }
+                if constexpr (EXTRA == 2) x = __fmaf_rn(-row.slope, __builtin_fabsf((float)(row.p - at.first[p] - (16 * kt + 4 * g + r))), x);
+                t[p][kt][r] = x;
             }
-    }
-    float most = t[0][0];
+        }
+        if (!whole) {
+            const int lo = row.lo - at.first[p], hi = row.hi - at.first[p];
 #pragma unroll
-    for (int i = 1; i < 16; ++i) most = fmaxf(most, t[i >> 2][i & 3]);
-    most = quad_max(most);
+            for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int j = 16 * kt + 4 * g + r;
+                    if (j < lo || j >= hi) t[p][kt][r] = -__builtin_inff();
+                }
+        }
+        float m = t[p][0][0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) m = fmaxf(m, t[p][i >> 2][i & 3]);
+        most_of[p] = quad_max(m);
+    }
+    keys_done();
+    float most = most_of[0];
+#pragma unroll
+    for (int p = 1; p < NP; ++p) most = fmaxf(most, most_of[p]);
     const bool sees = most != -__builtin_inff();
     const float base = sees ? most : 0.f;
-    float sum = 0.f;
-    v4i w[3];
+    // weights times value scales are at most `unit`
+    float unit = 0.f, times[NP];
+    if constexpr (NP == 1) unit = at.v_scale[0], times[0] = 0x1p22f;
+    else {
 #pragma unroll
-    for (int kt = 0; kt < 4; ++kt) {
-        unsigned u[4];
+        for (int p = 0; p < NP; ++p) unit = fmaxf(unit, __fmul_rn(fast_exp2(__fadd_rn(most_of[p], -base)), at.v_scale[p]));
+        // (finite whatever the scales: a page that the row does not see may have one that is far larger)
+        const float per = unit > 0.f ? fminf(__fdividef(0x1p22f, unit), 0x1p124f) : 0.f;
 #pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float e = fast_exp2(__fadd_rn(t[kt][r], -base));
-            sum = __fadd_rn(sum, e);
-            u[r] = __float_as_uint(__fmaf_rn(e, 0x1p22f, 8388608.f + 32896.f));  // 2^23 + 0x8080: the mantissa is the rounded number
-        }
-        int low, mid, high;
-        split_digits(u, low, mid, high);
-        w[2][kt] = low, w[1][kt] = mid, w[0][kt] = high;
+        for (int p = 0; p < NP; ++p) times[p] = fminf(__fmul_rn(at.v_scale[p], per), 0x1p126f);
     }
+    float sum = 0.f;
+    v4i w[NP][3];
+#pragma unroll
+    for (int p = 0; p < NP; ++p)
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) {
+            unsigned u[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float e = fast_exp2(__fadd_rn(t[p][kt][r], -base));
+                sum = __fadd_rn(sum, e);
+                u[r] = __float_as_uint(__fmaf_rn(e, times[p], 8388608.f + 32896.f));  // 2^23 + 0x8080: the mantissa is the rounded number
+            }
+            int low, mid, high;
+            split_digits(u, low, mid, high);
+            w[p][2][kt] = low, w[p][1][kt] = mid, w[p][0][kt] = high;
+        }
     const float m = fmaxf(s.m, most);
     const float keep = s.m == -__builtin_inff() ? 0.f : fast_exp2(__fadd_rn(s.m, -m));
     const float take = sees ? fast_exp2(__fadd_rn(most, -m)) : 0.f;
     s.m = m;
     s.l = __fmaf_rn(s.l, keep, __fmul_rn(sum, take));
-    const float put = __fmul_rn(__fmul_rn(take, 0x1p-22f), v_scale);
+    const float put = __fmul_rn(__fmul_rn(take, 0x1p-22f), unit);
+    if (!__all(keep == 1.f)) {  // (a maximum seldom grows once a few pages are in)
+#pragma unroll
+        for (int dt = 0; dt < 4 * KC; ++dt)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s.o[dt][r] = __fmul_rn(s.o[dt][r], keep);
+    }
 #pragma unroll
     for (int dt = 0; dt < 4 * KC; ++dt) {
-        const v4i v = *reinterpret_cast<const v4i*>(vp + dt * 1024);
-        v4i a[3];
+        v4i a[3] = {};
 #pragma unroll
-        for (int n = 0; n < 3; ++n) a[n] = mma(v, w[n], v4i{0, 0, 0, 0});
+        for (int p = 0; p < NP; ++p) {
+            const v4i v = value(p, dt);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) s.o[dt][r] = __fmaf_rn(join_digits(a[0][r], a[1][r], a[2][r]), put, __fmul_rn(s.o[dt][r], keep));
+            for (int n = 0; n < 3; ++n) a[n] = mma(v, w[p][n], a[n]);
+        }
+#pragma unroll
+        for (int r = 0; r < 4; ++r) s.o[dt][r] = __fmaf_rn(join_digits(a[0][r], a[1][r], a[2][r]), put, s.o[dt][r]);
     }
+    values_done();
 }
 
-// 64 rows a workgroup, one key head: each wave a tile of 16 of them, or, where a sequence has at most 32, 16 rows of which two or
-// four waves share the pages out between them and join what they have in LDS.
-template <int KC, bool EXTRA>
+// A sequence's pages as a wave walks them: their numbers come 64 at a time, one a lane.
+struct PageWalk {
+    const int32_t* table;
+    int from, to, ids;
+    __device__ int id(int pg) {  // pg: from, from + 1, ...
+        if (((pg - from) & 63) == 0) ids = table[min(pg + (int)(threadIdx.x & 63), to - 1)];
+        return __builtin_amdgcn_readlane(ids, (pg - from) & 63);
+    }
+};
+// Pages pg .. pg + NP - 1, those behind the last and those that are none of the pool as pages whose tokens nobody sees, whatever is read
+// in their place.
+template <int NP>
+__device__ __forceinline__ Pages<NP> pages_at(const KvView& c, int head, PageWalk& walk, int pg, const int8_t* (&kp)[NP], const int8_t* (&vp)[NP]) {
+    Pages<NP> at;
+    at.all = true;
+#pragma unroll
+    for (int n = 0; n < NP; ++n) {
+        const int id = pg + n < walk.to ? walk.id(pg + n) : -1;
+        const bool is = (unsigned)id < (unsigned)c.n_pages;
+        const int page = is ? id : 0;
+        kp[n] = c.k + c.at(page, head), vp[n] = c.v + c.at(page, head);
+        const size_t sc = (size_t)page * c.heads + head;
+        at.k_scale[n] = c.ks[sc], at.v_scale[n] = is ? c.vs[sc] : 0.f;
+        at.first[n] = is ? (pg + n) * KV_BLOCK : 1 << 30;
+        at.all = at.all && is;
+    }
+    return at;
+}
+
+// pages that a workgroup stages at a time: two (see attend_pages) where they fit LDS twice, for two workgroups a compute unit
+template <int KC>
+constexpr int kv_staged() { return KC <= 2 ? 2 : 1; }
+template <int KC>
+constexpr int kv_lds_bytes(bool staged) {
+    const int join = 4 * 16 * (64 * KC + 4) * 4 + 4 * 16 * 2 * 4, stage = 2 * kv_staged<KC>() * 8 * KC * 1024;
+    return staged && stage > join ? stage : join;
+}
+
+// 64 rows a workgroup, one key head. Where a sequence has more than 32 rows each wave has a tile of 16 of them; they all read the same
+// pages, which the workgroup stages through LDS, the next ones on their way meanwhile (STAGED; straight from the caches each wave
+// would bring in 16 KB for 192 matrix instructions, and wait for them half of its time). Where it has fewer, two or four waves share a tile's
+// pages out between them, each with its next page's keys and values on their way into registers, and join what they have in LDS.
+template <int KC, int EXTRA, bool STAGED>
 __global__ void __launch_bounds__(256) kv_attend_kernel(AttendArgs a) {
-    __shared__ __attribute__((aligned(16))) float joined[4][16][64 * KC + 4];
-    __shared__ float joined_ml[4][16][2];
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kv_lds_bytes<KC>(STAGED)];
+    typedef float JoinedRows[16][64 * KC + 4];
+    JoinedRows* const joined = reinterpret_cast<JoinedRows*>(lds);
+    typedef float JoinedSums[16][2];
+    JoinedSums* const joined_ml = reinterpret_cast<JoinedSums*>(lds + sizeof(JoinedRows) * 4);
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), g = lane >> 4;
+    const unsigned lane16 = (unsigned)lane * 16u;
     const int head = (int)(blockIdx.x % (unsigned)a.c.heads);
     const int tile = a.tiles - 1 - (int)(blockIdx.x / (unsigned)a.c.heads);  // (a causal prompt's last tiles have the most to read)
     const int i = kv_find(a.b.starts, a.b.n_seqs, a.b.n_tokens, a.group, 64, 1, tile);
     const KvSeq s = kv_sequence(a.b, i);
     const int row0 = (tile - kv_tile_base(a.b.starts, i, a.b.n_tokens, a.group, 64, 1)) * 64, rows = s.count * a.group;
     if (row0 < 0 || row0 >= rows) return;
-    const int tiles = (min(rows - row0, 64) + 15) >> 4;            // of 16 rows
-    const int shares = tiles == 1 ? 4 : tiles == 2 ? 2 : 1;        // waves that share a tile's pages
-    const int mine = wave / shares, share = wave % shares;         // (a fourth wave of three tiles has none: it joins the barriers)
+    const int tiles = (min(rows - row0, 64) + 15) >> 4;      // of 16 rows
+    const int shares = tiles == 1 ? 4 : tiles == 2 ? 2 : 1;  // waves that share a tile's pages
+    const int mine = wave / shares, share = wave % shares;   // (a fourth wave of three tiles has none: it joins the barriers)
     const bool works = mine < tiles;
     const int r = row0 + mine * 16 + (lane & 15);
     const int row = min(r, rows - 1), token = row / a.group, q_head = head * a.group + row % a.group;
     const int p = s.first + token;
     const size_t out_row = (size_t)(s.begin + token) * a.q_heads + q_head;
-    // positions that this row sees: [lo, hi)
+    // positions that a row at p sees: [lo, hi)
     const int stored = min(s.length, a.b.max_pages * KV_BLOCK);
-    const int hi = p < 0 ? 0 : a.causal ? min(stored, p + 1) : stored;
-    const int lo = a.window > 0 && p >= a.window ? p - a.window + 1 : 0;
+    const auto sees_to = [&](int p) { return p < 0 ? 0 : a.causal ? min(stored, p + 1) : stored; };
+    const auto sees_from = [&](int p) { return a.window > 0 && p >= a.window ? p - a.window + 1 : 0; };
+    RowView view{sees_from(p), sees_to(p), p, 0.f};
+    if constexpr (EXTRA == 2) view.slope = __fmul_rn(a.slopes[q_head], LOG2E);
+    // what the wave's rows see: rows are in the order of their tokens
+    const int first_hi = __builtin_amdgcn_readlane(view.hi, 0), last_hi = __builtin_amdgcn_readlane(view.hi, 15);
+    const int first_lo = __builtin_amdgcn_readlane(view.lo, 0), last_lo = __builtin_amdgcn_readlane(view.lo, 15);
 
     Running<KC> run;
     run.m = -__builtin_inff(), run.l = 0.f;
@@ -239,37 +341,92 @@ __global__ void __launch_bounds__(256) kv_attend_kernel(AttendArgs a) {
     for (int dt = 0; dt < 4 * KC; ++dt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) run.o[dt][e] = 0.f;
-    if (works) {
-        // what the wave's rows see: rows are in the order of their tokens
-        const int first_hi = __builtin_amdgcn_readlane(hi, 0), last_hi = __builtin_amdgcn_readlane(hi, 15);
-        const int first_lo = __builtin_amdgcn_readlane(lo, 0), last_lo = __builtin_amdgcn_readlane(lo, 15);
-        const int page0 = first_lo / KV_BLOCK, pages = max((last_hi + KV_BLOCK - 1) / KV_BLOCK - page0, 0);
-        const int parts = a.splits * shares, part = (int)blockIdx.y * shares + share;
-        const int each = (pages + parts - 1) / parts;
-        const int from = page0 + min(part * each, pages), to = page0 + min((part + 1) * each, pages);
-        if (from < to) {
-            Queries<KC> q;
-            const bool whole_rows = a.c.dim % 4 == 0 && a.q_stride % 4 == 0 && ((size_t)a.q & 15) == 0;
-            load_queries<KC>(q, a.q + (size_t)(s.begin + token) * a.q_stride + (size_t)q_head * a.c.dim, a.c.dim, whole_rows);
-            const float factor = __fmul_rn(q.unit, a.scale);
-            float slope = 0.f;
-            if constexpr (EXTRA) slope = a.slopes ? __fmul_rn(a.slopes[q_head], LOG2E) : 0.f;
-            const int32_t* const table = a.b.pages + (size_t)i * a.b.max_pages;
-            int ids = 0;
-            for (int pg = from; pg < to; ++pg) {
-                if (((pg - from) & 63) == 0) ids = table[min(pg + lane, to - 1)];
-                const int id = __builtin_amdgcn_readlane(ids, (pg - from) & 63);
-                if ((unsigned)id >= (unsigned)a.c.n_pages) continue;  // not a page: its tokens are not seen
-                const size_t at = a.c.at(id, head);
-                const size_t sc = (size_t)id * a.c.heads + head;
-                const int base = pg * KV_BLOCK;
-                const bool whole = base + KV_BLOCK <= first_hi && base >= last_lo;
-                attend_page<KC, EXTRA>(run, q, a.c.k + at + lane * 16, a.c.v + at + lane * 16, __fmul_rn(factor, a.c.ks[sc]), a.c.vs[sc], a.cap,
-                                       slope, lo - base, hi - base, p - base, whole);
+    PageWalk walk;
+    walk.table = a.b.pages + (size_t)i * a.b.max_pages;
+    // pages [begin, end) of positions [lo, hi), the part-th of `parts` equal shares
+    const auto deal = [&](int lo, int hi, int part, int parts) {
+        const int page0 = lo / KV_BLOCK, pages = max((hi + KV_BLOCK - 1) / KV_BLOCK - page0, 0), each = (pages + parts - 1) / parts;
+        walk.from = page0 + min(part * each, pages), walk.to = page0 + min((part + 1) * each, pages);
+    };
+    Queries<KC> q;
+    float factor = 0.f;
+    const auto load_rows = [&] {
+        const bool whole_rows = a.c.dim % 4 == 0 && a.q_stride % 4 == 0 && ((size_t)a.q & 15) == 0;
+        load_queries<KC>(q, a.q + (size_t)(s.begin + token) * a.q_stride + (size_t)q_head * a.c.dim, a.c.dim, whole_rows);
+        factor = __fmul_rn(q.unit, a.scale);
+    };
+    const auto nothing = [] {};
+    if (STAGED && shares == 1) {
+        constexpr int NP = kv_staged<KC>(), TILES = NP * 8 * KC, MINE = TILES / 4;
+        v4i* const buffer = reinterpret_cast<v4i*>(lds);  // [2][page][4 KC tiles of keys, as many of values][lane]
+        const int p0 = s.first + row0 / a.group, p1 = s.first + (min(row0 + 64, rows) - 1) / a.group;
+        deal(sees_from(p0), sees_to(p1), (int)blockIdx.y, a.splits);
+        if (walk.from < walk.to) {
+            load_rows();
+            v4i mine_of[MINE];
+            Pages<NP> at, next;
+            const auto load = [&](int pg) {
+                const int8_t *kp[NP], *vp[NP];
+                next = pages_at<NP>(a.c, head, walk, pg, kp, vp);
+#pragma unroll
+                for (int u = 0; u < MINE; ++u) {
+                    const int j = wave * MINE + u, n = j / (8 * KC), of = j % (8 * KC);
+                    const int8_t* const k = NP == 2 && n ? kp[NP - 1] : kp[0];
+                    const int8_t* const v = NP == 2 && n ? vp[NP - 1] : vp[0];
+                    mine_of[u] = *reinterpret_cast<const v4i*>((of < 4 * KC ? k + of * 1024 : v + (of - 4 * KC) * 1024) + lane16);
+                }
+            };
+            const auto put = [&](int half) {
+#pragma unroll
+                for (int u = 0; u < MINE; ++u) buffer[(half * TILES + wave * MINE + u) * 64 + lane] = mine_of[u];
+            };
+            load(walk.from);
+            put(0);
+            for (int pg = walk.from, half = 0; pg < walk.to; pg += NP, half ^= 1) {
+                at = next;
+                if (pg + NP < walk.to) load(pg + NP);
+                // these pages are in LDS, and nobody reads the other half any more (loads from memory stay in flight)
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                if (works && pg * KV_BLOCK < last_hi && (pg + NP) * KV_BLOCK > first_lo) {
+                    const bool whole = at.all && (pg + NP) * KV_BLOCK <= first_hi && pg * KV_BLOCK >= last_lo;
+                    const v4i* const from = buffer + half * TILES * 64 + lane;
+                    attend_pages<KC, EXTRA, NP>(
+                        run, q, [&](int n, int tile) { return from[(n * 8 * KC + tile) * 64]; },
+                        [&](int n, int tile) { return from[(n * 8 * KC + 4 * KC + tile) * 64]; }, nothing, nothing, at, factor, a.cap, view, whole);
+                }
+                if (pg + NP < walk.to) put(half ^ 1);
             }
         }
-        run.l = quad_sum(run.l);
+    } else if (works) {
+        deal(first_lo, last_hi, (int)blockIdx.y * shares + share, a.splits * shares);
+        if (walk.from < walk.to) {
+            load_rows();
+            v4i keys[4 * KC], values[4 * KC];
+            const int8_t *kp[1], *vp[1];
+            Pages<1> at = pages_at<1>(a.c, head, walk, walk.from, kp, vp);
+            const auto load = [&](v4i (&to)[4 * KC], const int8_t* page) {
+#pragma unroll
+                for (int n = 0; n < 4 * KC; ++n) to[n] = *reinterpret_cast<const v4i*>(page + n * 1024 + lane16);
+                __builtin_amdgcn_sched_barrier(0);  // (they are asked for here, not where they are used)
+            };
+            load(keys, kp[0]);
+            load(values, vp[0]);
+            const auto page = [&](int pg, const auto& keys_done, const auto& values_done) {
+                const bool whole = at.all && (pg + 1) * KV_BLOCK <= first_hi && pg * KV_BLOCK >= last_lo;
+                attend_pages<KC, EXTRA, 1>(
+                    run, q, [&](int, int tile) { return keys[tile]; }, [&](int, int tile) { return values[tile]; }, keys_done, values_done, at, factor,
+                    a.cap, view, whole);
+            };
+            int pg = walk.from;
+            for (; pg + 1 < walk.to; ++pg) {
+                const Pages<1> next = pages_at<1>(a.c, head, walk, pg + 1, kp, vp);
+                page(pg, [&] { load(keys, kp[0]); }, [&] { load(values, vp[0]); });
+                at = next;
+            }
+            page(pg, nothing, nothing);
+        }
     }
+    run.l = quad_sum(run.l);
     if (shares > 1) {
         if (works) {
 #pragma unroll
@@ -397,10 +554,17 @@ int kv_attend_splits(int tiles, int heads, int max_pages) {
 }
 int kv_attend_tiles(int n_tokens, int n_seqs, int group) { return (int)((size_t)n_tokens * group / 64) + n_seqs; }
 
+template <int KC, bool STAGED>
+static void launch_attend(const AttendArgs& a, dim3 grid, hipStream_t stream) {
+    if (a.slopes) launch(kv_attend_kernel<KC, 2, STAGED>, grid, dim3(256), 0, stream, a);
+    else if (a.cap != 0.f) launch(kv_attend_kernel<KC, 1, STAGED>, grid, dim3(256), 0, stream, a);
+    else launch(kv_attend_kernel<KC, 0, STAGED>, grid, dim3(256), 0, stream, a);
+}
 template <int KC>
-static void launch_attend(const AttendArgs& a, bool extra, dim3 grid, hipStream_t stream) {
-    if (extra) launch(kv_attend_kernel<KC, true>, grid, dim3(256), 0, stream, a);
-    else launch(kv_attend_kernel<KC, false>, grid, dim3(256), 0, stream, a);
+static void launch_attend(const AttendArgs& a, dim3 grid, hipStream_t stream) {
+    // (staging is for workgroups of more than 32 rows, and LDS for it keeps others out: by the average of the sequences)
+    if ((size_t)a.b.n_tokens * a.group > 32 * (size_t)a.b.n_seqs) launch_attend<KC, true>(a, grid, stream);
+    else launch_attend<KC, false>(a, grid, stream);
 }
 
 hipError_t run_kv_attend(const KvView& c, const KvBatch& b, const float* q, size_t q_stride, float* out, int q_heads, float scale, float cap,
@@ -415,12 +579,11 @@ hipError_t run_kv_attend(const KvView& c, const KvBatch& b, const float* q, size
     a.part_ml = (float*)workspace;
     a.part_o = a.part_ml + (splits > 1 ? (2 * rows * splits + 3) / 4 * 4 : 0);
     const dim3 grid((unsigned)a.tiles * (unsigned)c.heads, (unsigned)splits);
-    const bool extra = cap != 0.f || slopes != nullptr;
     switch (c.chunks) {
-    case 1: launch_attend<1>(a, extra, grid, stream); break;
-    case 2: launch_attend<2>(a, extra, grid, stream); break;
-    case 3: launch_attend<3>(a, extra, grid, stream); break;
-    default: launch_attend<4>(a, extra, grid, stream); break;
+    case 1: launch_attend<1>(a, grid, stream); break;
+    case 2: launch_attend<2>(a, grid, stream); break;
+    case 3: launch_attend<3>(a, grid, stream); break;
+    default: launch_attend<4>(a, grid, stream); break;
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || splits == 1) return e;
