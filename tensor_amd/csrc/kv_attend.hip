@@ -51,8 +51,8 @@ __device__ __forceinline__ float quad_sum(float x) {
 }
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// tanh of scores that are at most a few thousand: 1 - 2 / (exp(2 x) + 1) loses the bits of a small x, where the series goes on to x^9
-// (|x| < 1/4: the next term is below 2^-27 x).
+// tanh. 1 - 2 / (exp(2 x) + 1) loses the bits of a small x, where the series goes on (to x^9 below 1/4, where the next term is under
+// 2^-26 of x; to x^13 below 1/2).
 __device__ __forceinline__ float tanh_of(float x) {
     const float a = __builtin_fabsf(x), y = __fmul_rn(x, x);
     const float big = __fmaf_rn(-2.f, __fdividef(1.f, __fadd_rn(fast_exp2(__fmul_rn(a, 2.f * LOG2E)), 1.f)), 1.f);
@@ -61,6 +61,15 @@ __device__ __forceinline__ float tanh_of(float x) {
     s = __fmaf_rn(y, s, -1.f / 3.f);
     s = __fmaf_rn(__fmul_rn(y, a), s, a);
     return __builtin_copysignf(a < 0.25f ? s : big, x);
+}
+__device__ __forceinline__ float tanh_of_half(float x) {  // |x| < 1/2
+    const float y = __fmul_rn(x, x);
+    float s = __fmaf_rn(y, 21844.f / 6081075.f, -1382.f / 155925.f);
+    s = __fmaf_rn(y, s, 62.f / 2835.f);
+    s = __fmaf_rn(y, s, -17.f / 315.f);
+    s = __fmaf_rn(y, s, 2.f / 15.f);
+    s = __fmaf_rn(y, s, -1.f / 3.f);
+    return __fmaf_rn(__fmul_rn(y, x), s, x);
 }
 
 // Three signed digits of four fixed-point numbers (u = number + 0x8080 in the low 24 bits): u's low two bytes less 128, and the third.
@@ -84,9 +93,9 @@ struct Queries {
     float unit;        // what 1 stands for (NaN: the row holds a NaN or an infinity)
 };
 
-// A lane's share of its row: 16 dims of every 64.
+// A lane's share of its row: 16 dims of every 64; `negative`: of the row times -1 (the units are never negative).
 template <int KC>
-__device__ __forceinline__ void load_queries(Queries<KC>& q, const float* __restrict__ row, int dim, bool whole) {
+__device__ __forceinline__ void load_queries(Queries<KC>& q, const float* __restrict__ row, int dim, bool whole, bool negative) {
     const int g = (int)(threadIdx.x >> 4) & 3;
     float x[KC][16];
     float most = 0.f;
@@ -117,7 +126,7 @@ __device__ __forceinline__ void load_queries(Queries<KC>& q, const float* __rest
     // units of 2^(e - 21), most in [2^e, 2^(e + 1)): at most 2^22 of them. (A row below 2^-100 counts as 0.)
     const int e = (int)(__float_as_uint(most) >> 23) - 127;
     const bool none = odd || e < -100;
-    const float per = none ? 0.f : __uint_as_float((unsigned)(127 + 21 - e) << 23);
+    const float size = none ? 0.f : __uint_as_float((unsigned)(127 + 21 - e) << 23), per = negative ? -size : size;
     q.unit = odd ? __builtin_nanf("") : none ? 0.f : __uint_as_float((unsigned)(127 - 21 + e) << 23);
 #pragma unroll
     for (int c = 0; c < KC; ++c)
@@ -161,10 +170,12 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
                                              const ValuesDone& values_done, const Pages<NP>& at, float factor, float cap, const RowView& row,
                                              bool whole) {
     const int g = (int)(threadIdx.x >> 4) & 3;
-    float t[NP][4][4], most_of[NP];
+    // scores (log2) are t * unit_of; without cap and slopes the product is left to the subtraction of the maximum
+    float t[NP][4][4], most_of[NP], unit_of[NP];
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
-        const float unit = __fmul_rn(factor, at.k_scale[p]);  // of the page's scores, log2
+        const float unit = __fmul_rn(factor, at.k_scale[p]);
+        unit_of[p] = EXTRA == 0 ? unit : 1.f;
 #pragma unroll
         for (int kt = 0; kt < 4; ++kt) {
             v4i a[3] = {};
@@ -176,13 +187,28 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float x = __fmul_rn(join_digits(a[0][r], a[1][r], a[2][r]), unit);
-                if constexpr (EXTRA != 0) {
-                    if (EXTRA == 1 || cap != 0.f) x = __fmul_rn(tanh_of(x), cap);
-                }
-                if constexpr (EXTRA == 2) x = __fmaf_rn(-row.slope, __builtin_fabsf((float)(row.p - at.first[p] - (16 * kt + 4 * g + r))), x);
-                t[p][kt][r] = x;
+                float x = join_digits(a[0][r], a[1][r], a[2][r]);
+                t[p][kt][r] = EXTRA == 0 ? x : __fmul_rn(x, unit);
             }
+        }
+        if (EXTRA == 1 || (EXTRA == 2 && cap != 0.f)) {
+            // most scores are far below the cap: a third of the instructions for a page where all are below half of it
+            float far = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) far = fmaxf(far, __builtin_fabsf(t[p][i >> 2][i & 3]));
+            if (__all(far < 0.5f)) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) t[p][i >> 2][i & 3] = __fmul_rn(tanh_of_half(t[p][i >> 2][i & 3]), cap);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) t[p][i >> 2][i & 3] = __fmul_rn(tanh_of(t[p][i >> 2][i & 3]), cap);
+            }
+        }
+        if constexpr (EXTRA == 2) {
+            const float away = (float)(row.p - at.first[p] - 4 * g);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                t[p][i >> 2][i & 3] = __fmaf_rn(-row.slope, __builtin_fabsf(__fadd_rn(away, -(float)(16 * (i >> 2) + (i & 3)))), t[p][i >> 2][i & 3]);
         }
         if (!whole) {
             const int lo = row.lo - at.first[p], hi = row.hi - at.first[p];
@@ -191,13 +217,14 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int j = 16 * kt + 4 * g + r;
-                    if (j < lo || j >= hi) t[p][kt][r] = -__builtin_inff();
+                    t[p][kt][r] = j < lo || j >= hi ? -__builtin_inff() : __fmul_rn(t[p][kt][r], unit_of[p]);
                 }
+            unit_of[p] = 1.f;
         }
         float m = t[p][0][0];
 #pragma unroll
         for (int i = 1; i < 16; ++i) m = fmaxf(m, t[p][i >> 2][i & 3]);
-        most_of[p] = quad_max(m);
+        most_of[p] = __fmul_rn(quad_max(m), unit_of[p]);
     }
     keys_done();
     float most = most_of[0];
@@ -216,6 +243,16 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
 #pragma unroll
         for (int p = 0; p < NP; ++p) times[p] = fminf(__fmul_rn(at.v_scale[p], per), 0x1p126f);
     }
+    // The exact product less the rounded maximum can be above 0, by 2^-24 of it. Up to 2^22 the weights' three digits have room for that;
+    // scores beyond are rounded first.
+    if (EXTRA == 0 && __any(__builtin_fabsf(base) > 0x1p22f)) {
+#pragma unroll
+        for (int p = 0; p < NP; ++p) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) t[p][i >> 2][i & 3] = __fmul_rn(t[p][i >> 2][i & 3], unit_of[p]);
+            unit_of[p] = 1.f;
+        }
+    }
     float sum = 0.f;
     v4i w[NP][3];
 #pragma unroll
@@ -225,7 +262,7 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
             unsigned u[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const float e = fast_exp2(__fadd_rn(t[p][kt][r], -base));
+                const float e = fast_exp2(__fmaf_rn(t[p][kt][r], unit_of[p], -base));
                 sum = __fadd_rn(sum, e);
                 u[r] = __float_as_uint(__fmaf_rn(e, times[p], 8388608.f + 32896.f));  // 2^23 + 0x8080: the mantissa is the rounded number
             }
@@ -289,21 +326,25 @@ __device__ __forceinline__ Pages<NP> pages_at(const KvView& c, int head, PageWal
     return at;
 }
 
-// pages that a workgroup stages at a time: two (see attend_pages) where they fit LDS twice, for two workgroups a compute unit
+// waves a SIMD that the launch is compiled for: three where that costs no more than a dozen registers spilled (4096 rows on 14 k tokens of
+// 128 dims: 1.33 ms with three, 1.46 with two and two buffers in LDS)
+template <int KC, int EXTRA>
+constexpr int kv_waves(bool staged) { return !staged || KC > 2 ? 1 : KC == 1 || EXTRA == 0 ? 3 : 2; }
+// pages that a workgroup stages at a time: two (see attend_pages) where that leaves LDS for three workgroups a compute unit
 template <int KC>
 constexpr int kv_staged() { return KC <= 2 ? 2 : 1; }
 template <int KC>
 constexpr int kv_lds_bytes(bool staged) {
-    const int join = 4 * 16 * (64 * KC + 4) * 4 + 4 * 16 * 2 * 4, stage = 2 * kv_staged<KC>() * 8 * KC * 1024;
+    const int join = 4 * 16 * (64 * KC + 4) * 4 + 4 * 16 * 2 * 4, stage = kv_staged<KC>() * 8 * KC * 1024;
     return staged && stage > join ? stage : join;
 }
 
 // 64 rows a workgroup, one key head. Where a sequence has more than 32 rows each wave has a tile of 16 of them; they all read the same
-// pages, which the workgroup stages through LDS, the next ones on their way meanwhile (STAGED; straight from the caches each wave
-// would bring in 16 KB for 192 matrix instructions, and wait for them half of its time). Where it has fewer, two or four waves share a tile's
+// pages, which the workgroup stages through LDS, the next ones on their way into registers meanwhile (STAGED; straight from the caches each
+// wave would bring in 16 KB for 48 matrix instructions, and wait for them half of its time). Where it has fewer, two or four waves share a tile's
 // pages out between them, each with its next page's keys and values on their way into registers, and join what they have in LDS.
 template <int KC, int EXTRA, bool STAGED>
-__global__ void __launch_bounds__(256) kv_attend_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(256, (kv_waves<KC, EXTRA>(STAGED))) kv_attend_kernel(AttendArgs a) {
     __shared__ __attribute__((aligned(16))) unsigned char lds[kv_lds_bytes<KC>(STAGED)];
     typedef float JoinedRows[16][64 * KC + 4];
     JoinedRows* const joined = reinterpret_cast<JoinedRows*>(lds);
@@ -352,13 +393,13 @@ __global__ void __launch_bounds__(256) kv_attend_kernel(AttendArgs a) {
     float factor = 0.f;
     const auto load_rows = [&] {
         const bool whole_rows = a.c.dim % 4 == 0 && a.q_stride % 4 == 0 && ((size_t)a.q & 15) == 0;
-        load_queries<KC>(q, a.q + (size_t)(s.begin + token) * a.q_stride + (size_t)q_head * a.c.dim, a.c.dim, whole_rows);
-        factor = __fmul_rn(q.unit, a.scale);
+        load_queries<KC>(q, a.q + (size_t)(s.begin + token) * a.q_stride + (size_t)q_head * a.c.dim, a.c.dim, whole_rows, a.scale < 0.f);
+        factor = __fmul_rn(q.unit, __builtin_fabsf(a.scale));
     };
     const auto nothing = [] {};
     if (STAGED && shares == 1) {
         constexpr int NP = kv_staged<KC>(), TILES = NP * 8 * KC, MINE = TILES / 4;
-        v4i* const buffer = reinterpret_cast<v4i*>(lds);  // [2][page][4 KC tiles of keys, as many of values][lane]
+        v4i* const buffer = reinterpret_cast<v4i*>(lds);  // [page][4 KC tiles of keys, as many of values][lane]
         const int p0 = s.first + row0 / a.group, p1 = s.first + (min(row0 + 64, rows) - 1) / a.group;
         deal(sees_from(p0), sees_to(p1), (int)blockIdx.y, a.splits);
         if (walk.from < walk.to) {
@@ -376,25 +417,25 @@ __global__ void __launch_bounds__(256) kv_attend_kernel(AttendArgs a) {
                     mine_of[u] = *reinterpret_cast<const v4i*>((of < 4 * KC ? k + of * 1024 : v + (of - 4 * KC) * 1024) + lane16);
                 }
             };
-            const auto put = [&](int half) {
+            const auto put = [&] {
 #pragma unroll
-                for (int u = 0; u < MINE; ++u) buffer[(half * TILES + wave * MINE + u) * 64 + lane] = mine_of[u];
+                for (int u = 0; u < MINE; ++u) buffer[(wave * MINE + u) * 64 + lane] = mine_of[u];
             };
             load(walk.from);
-            put(0);
-            for (int pg = walk.from, half = 0; pg < walk.to; pg += NP, half ^= 1) {
+            for (int pg = walk.from; pg < walk.to; pg += NP) {
                 at = next;
+                put();
                 if (pg + NP < walk.to) load(pg + NP);
-                // these pages are in LDS, and nobody reads the other half any more (loads from memory stay in flight)
+                // these pages are in LDS (loads from memory stay in flight)
                 asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 if (works && pg * KV_BLOCK < last_hi && (pg + NP) * KV_BLOCK > first_lo) {
                     const bool whole = at.all && (pg + NP) * KV_BLOCK <= first_hi && pg * KV_BLOCK >= last_lo;
-                    const v4i* const from = buffer + half * TILES * 64 + lane;
+                    const v4i* const from = buffer + lane;
                     attend_pages<KC, EXTRA, NP>(
                         run, q, [&](int n, int tile) { return from[(n * 8 * KC + tile) * 64]; },
                         [&](int n, int tile) { return from[(n * 8 * KC + 4 * KC + tile) * 64]; }, nothing, nothing, at, factor, a.cap, view, whole);
                 }
-                if (pg + NP < walk.to) put(half ^ 1);
+                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // nobody reads them any more
             }
         }
     } else if (works) {

@@ -182,6 +182,52 @@ def test_attend_of_long_caches(hip, dim, lengths):
         s.check_attend(s.now, s.normal(s.now, 1, 3)[0], **kw)
 
 
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+@pytest.mark.parametrize("lengths", [[(70 * i, 1) for i in range(20)] + [(300, 90)], [(0, 400), (1000, 30)], [(500, 33), (5, 17), (0, 300)]])
+def test_attend_of_few_and_many_rows_together(hip, dim, lengths):
+    """Sequences of every kind beside each other, in the launch for many rows and in that for few: which one it is follows from the
+    average. Two query heads: 16, 32, 48 rows and 64 at a time; pages in odd numbers; a page in the middle that is none."""
+    s = Setup(hip, np.random.default_rng(21 + dim), 1, dim, lengths, front=1, behind=2)
+    s.append(s.now, *s.normal(s.now, 2))
+    for kw in (dict(), dict(window=130), dict(cap=4.0), dict(causal=False), dict(cap=60.0, slopes=np.array([0.05, 0.3], np.float32))):
+        s.check_attend(s.now, s.normal(s.now, 1, 2)[0], **kw)
+    s.table[-1, 2] = s.pages
+    s.check_attend(s.batch([n for _, n in lengths], [o + n for o, n in lengths], 1, 2), s.normal(s.now, 1, 2)[0])
+
+
+def test_attend_of_scores_beyond_all_measure(hip):
+    """Scores up to 2^30, where the largest takes it all, beside others within rounding of nothing."""
+    rng = np.random.default_rng(22)
+    for size in (2.0 ** 10, 2.0 ** 18, 2.0 ** 22):
+        s = Setup(hip, rng, 1, 128, [(0, 300)])
+        k, v = s.normal(s.now, 2)
+        s.append(s.now, k, v)
+        into = np.zeros((300, 1, 128), np.float32)
+        q = (k * np.float32(size)).astype(np.float32)
+        out = s.cache.attend(s.now[3], hip.to_device(q), scale=1.0).cpu().numpy()
+        values = s.model.read(s.now[0], s.now[1], s.table, (k, v))[1]
+        # a token's own key is far ahead of every other's: 128 against at most 60 times `size`
+        np.testing.assert_allclose(out, values, rtol=2.0 ** -20, atol=2.0 ** -20 * np.abs(values).max())
+
+
+def test_pages_of_very_different_size(hip):
+    """Value scales from 2^-99 to 2^100 beside each other, zeros among them: a page's share is rounded to the largest share of its step,
+    not to the largest scale."""
+    rng = np.random.default_rng(23)
+    n = 64 * 8
+    for dim in (64, 128):
+        s = Setup(hip, rng, 1, dim, [(0, n)])
+        k, v = s.normal(s.now, 2)
+        for i, e in enumerate([0, -99, 3, None, -60, 40, 0, 100]):
+            v[64 * i:64 * i + 64] *= np.float32(0 if e is None else 2.0 ** e)
+        s.append(s.now, k, v)
+        # rows up to the fifth page: nothing larger than the third's is in sight, and bounds are in terms of what is
+        b = s.batch([300], [300])
+        s.check_attend(b, s.normal(b, 1, 2)[0])
+        s.check_attend(b, s.normal(b, 1, 2)[0], window=70)
+        s.check_attend(s.now, s.normal(s.now, 1, 2)[0])
+
+
 def test_attend_with_pages_far_from_each_other(hip):
     """One token of a page outweighs thousands of the others, and the largest score comes first, last and in between: the running
     maximum, and the weights of pages that hold little."""
