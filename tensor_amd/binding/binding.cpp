@@ -13,9 +13,13 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/record_function.h>
+#include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/LocalDispatchKeySet.h>
 #include <c10/hip/HIPStream.h>
 
+#include <climits>
+#include <cmath>
+#include <initializer_list>
 #include <stdexcept>
 #include <string>
 
@@ -68,13 +72,14 @@ struct Args {
 
 // An allocation. The dispatcher in front of it costs 0.5 us of a call's 4.6, so it is left out where nothing can be listening: no
 // dispatch mode or transform of this thread, no profiler, and no deterministic filling of new memory.
-at::Tensor device_empty(int64_t count, at::ScalarType dt, long device) {
+at::Tensor device_empty(at::IntArrayRef shape, at::ScalarType dt, long device) {
     const c10::Device where(c10::DeviceType::CUDA, (c10::DeviceIndex)device);
     if (c10::impl::tls_local_dispatch_key_set().included_ == c10::default_included_set && !at::hasCallbacks() &&
         !at::globalContext().deterministicAlgorithms())
-        return at::detail::empty_cuda({count}, dt, where, std::nullopt);
-    return at::empty({count}, at::TensorOptions().dtype(dt).device(where));
+        return at::detail::empty_cuda(shape, dt, where, std::nullopt);
+    return at::empty(shape, at::TensorOptions().dtype(dt).device(where));
 }
+at::Tensor device_empty(int64_t count, at::ScalarType dt, long device) { return device_empty(at::IntArrayRef{count}, dt, device); }
 at::ScalarType type_of_layout(int layout) {
     return layout <= OTTER_HIP_F32_P8 ? at::kFloat : layout <= OTTER_HIP_I8_P8 ? at::kChar : at::kInt;
 }
@@ -289,6 +294,186 @@ PyObject* conv_block(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
     }
 }
 
+// What the transformer layers are handed is checked here, as they are called once a layer too: a tensor of type `dt` on the GPU
+// `device` with these sizes (-1: any), contiguous, with `rows` but for its first stride. The text of what is wrong, or null.
+const char* not_as(const at::Tensor* t, at::ScalarType dt, long device, std::initializer_list<int64_t> sizes, bool rows = false) {
+    if (!t) return "a tensor expected";
+    if (t->layout() != at::kStrided || !t->is_cuda() || t->get_device() != device) return "a tensor on the library's GPU expected";
+    if (t->scalar_type() != dt) return dt == at::kFloat ? "a float32 tensor expected" : "an int32 tensor expected";
+    if (t->dim() != (int64_t)sizes.size()) return "wrong number of dimensions";
+    int64_t d = 0;
+    for (const int64_t n : sizes) {
+        if (n >= 0 && t->size(d) != n) return "wrong shape";
+        ++d;
+    }
+    if (t->numel() == 0) return nullptr;
+    int64_t stride = 1;
+    for (d = t->dim() - 1; d >= (rows ? 1 : 0); --d) {
+        if (t->size(d) != 1 && t->stride(d) != stride) return "not contiguous";
+        stride *= t->size(d);
+    }
+    return nullptr;
+}
+PyObject* refuse(const char* call, const char* what, const char* why) {
+    PyObject* args = Py_BuildValue("(iN)", OTTER_HIP_ERR_INVALID, PyUnicode_FromFormat("%s: %s: %s", call, what, why));
+    if (args) PyErr_SetObject(g_error ? g_error : PyExc_RuntimeError, args);
+    Py_XDECREF(args);
+    return nullptr;
+}
+#define AS(call, what, ...)                                                           \
+    if (const char* why = not_as(__VA_ARGS__)) return refuse(call, what, why);
+
+// (otter_hip_kv_cache*, otter_hip_kv_batch*, keys, values, device)
+PyObject* kv_append(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    NEED(5)
+    try {
+        Args g{a};
+        const auto* c = g.handle<otter_hip_kv_cache>(0);
+        const auto* b = g.handle<otter_hip_kv_batch>(1);
+        const long device = g.num(4);
+        if (!g.ok) return nullptr;
+        const at::Tensor *k = THPVariable_Check(a[2]) ? g.tensor(2) : nullptr, *v = THPVariable_Check(a[3]) ? g.tensor(3) : nullptr;
+        AS("kv_append", "keys", k, at::kFloat, device, {b->n_tokens, c->heads, c->head_dim}, true)
+        AS("kv_append", "values", v, at::kFloat, device, {b->n_tokens, c->heads, c->head_dim}, true)
+        const c10::DeviceGuard on(c10::Device(c10::DeviceType::CUDA, (c10::DeviceIndex)device));
+        void* stream = stream_now();
+        const float *pk = (const float*)k->data_ptr(), *pv = (const float*)v->data_ptr();
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = otter_hip_kv_append(c, b, pk, (size_t)k->stride(0), pv, (size_t)v->stride(0), stream);
+        Py_END_ALLOW_THREADS
+        if (rc) return raise_status(rc);
+        Py_RETURN_NONE;
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
+}
+
+// (otter_hip_kv_cache*, otter_hip_kv_batch*, keys or None, values or None, device) -> (keys, values)
+PyObject* kv_read(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    NEED(5)
+    try {
+        Args g{a};
+        const auto* c = g.handle<otter_hip_kv_cache>(0);
+        const auto* b = g.handle<otter_hip_kv_batch>(1);
+        const at::Tensor *k = g.tensor(2), *v = g.tensor(3);
+        const long device = g.num(4);
+        if (!g.ok) return nullptr;
+        if (k) AS("kv_read", "keys", k, at::kFloat, device, {b->n_tokens, c->heads, c->head_dim})
+        if (v) AS("kv_read", "values", v, at::kFloat, device, {b->n_tokens, c->heads, c->head_dim})
+        const c10::DeviceGuard on(c10::Device(c10::DeviceType::CUDA, (c10::DeviceIndex)device));
+        at::Tensor made_k, made_v;
+        const int64_t shape[3] = {b->n_tokens, c->heads, c->head_dim};
+        if (!k) k = &(made_k = device_empty(at::IntArrayRef(shape, 3), at::kFloat, device));
+        if (!v) v = &(made_v = device_empty(at::IntArrayRef(shape, 3), at::kFloat, device));
+        void* stream = stream_now();
+        float *pk = (float*)k->data_ptr(), *pv = (float*)v->data_ptr();
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = otter_hip_kv_read(c, b, pk, pv, stream);
+        Py_END_ALLOW_THREADS
+        if (rc) return raise_status(rc);
+        PyObject *ko = result(a[2], *k), *vo = result(a[3], *v);
+        PyObject* pair = ko && vo ? PyTuple_Pack(2, ko, vo) : nullptr;
+        Py_XDECREF(ko), Py_XDECREF(vo);
+        return pair;
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
+}
+
+// (otter_hip_kv_cache*, otter_hip_kv_batch*, q, scale or None, cap, causal, window, slopes or None, out or None, workspace or None, device)
+PyObject* kv_attend(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    NEED(11)
+    try {
+        Args g{a};
+        const auto* c = g.handle<otter_hip_kv_cache>(0);
+        const auto* b = g.handle<otter_hip_kv_batch>(1);
+        const at::Tensor* q = g.tensor(2);
+        otter_hip_kv_attend_desc d{};
+        if (!g.ok) return nullptr;
+        d.scale = a[3] == Py_None ? (float)(1.0 / std::sqrt((double)c->head_dim)) : (float)g.real(3);
+        d.cap = (float)g.real(4);
+        d.causal = PyObject_IsTrue(a[5]);
+        const long window = g.num(6);
+        d.window = window > INT_MAX ? INT_MAX : window < 0 ? -1 : (int)window;
+        const at::Tensor *slopes = g.tensor(7), *out = g.tensor(8), *ws = g.tensor(9);
+        const long device = g.num(10);
+        if (!g.ok || d.causal < 0) return nullptr;
+        AS("kv_attend", "q", q, at::kFloat, device, {b->n_tokens, -1, c->head_dim}, true)
+        d.q_heads = (int)q->size(1);
+        if (slopes) {
+            AS("kv_attend", "slopes", slopes, at::kFloat, device, {d.q_heads})
+            d.slopes = (const float*)slopes->data_ptr();
+        }
+        if (out) AS("kv_attend", "out", out, at::kFloat, device, {b->n_tokens, d.q_heads, c->head_dim})
+        const c10::DeviceGuard on(c10::Device(c10::DeviceType::CUDA, (c10::DeviceIndex)device));
+        at::Tensor made, made_ws;
+        if (!out) out = &(made = device_empty(q->sizes(), at::kFloat, device));
+        if (!ws) {
+            const size_t need = otter_hip_kv_attend_workspace_bytes(c, b, &d);
+            if (need) ws = &(made_ws = device_empty((int64_t)need, at::kChar, device));
+        }
+        void* stream = stream_now();
+        const float* pq = (const float*)q->data_ptr();
+        void *po = out->data_ptr(), *pw = ws ? ws->data_ptr() : nullptr;
+        const size_t wb = ws ? bytes_of(*ws) : 0;
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = otter_hip_kv_attend(c, b, &d, pq, (size_t)q->stride(0), (float*)po, pw, wb, stream);
+        Py_END_ALLOW_THREADS
+        if (rc) return raise_status(rc);
+        return result(a[8], *out);
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
+}
+
+// (handle, experts, in_features, out_features, x, starts or None, index or None, out or None, workspace or None, device)
+PyObject* linear_forward(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
+    NEED(10)
+    try {
+        Args g{a};
+        auto* h = g.handle<otter_hip_linear_t>(0);
+        const long experts = g.num(1), in = g.num(2), columns = g.num(3);
+        const at::Tensor *x = g.tensor(4), *starts = g.tensor(5), *index = g.tensor(6), *out = g.tensor(7), *ws = g.tensor(8);
+        const long device = g.num(9);
+        if (!g.ok) return nullptr;
+        AS("linear", "x", x, at::kFloat, device, {-1, in}, true)
+        if (index) AS("linear", "index", index, at::kInt, device, {-1})
+        if (starts) AS("linear", "starts", starts, at::kInt, device, {experts + 1})
+        const int64_t shape[2] = {index ? index->size(0) : x->size(0), columns};
+        if (out) AS("linear", "out", out, at::kFloat, device, {shape[0], columns})
+        if (x->size(0) > INT_MAX || shape[0] > INT_MAX) return refuse("linear", "x", "too many rows");
+        const int x_rows = (int)x->size(0), rows = (int)shape[0];
+        const c10::DeviceGuard on(c10::Device(c10::DeviceType::CUDA, (c10::DeviceIndex)device));
+        at::Tensor made, made_ws;
+        if (!out) out = &(made = device_empty(at::IntArrayRef(shape, 2), at::kFloat, device));
+        if (!ws) {
+            const size_t need = otter_hip_linear_workspace_bytes(h, x_rows, rows);
+            if (need) ws = &(made_ws = device_empty((int64_t)need, at::kChar, device));
+        }
+        void* stream = stream_now();
+        const float* px = (const float*)x->data_ptr();
+        const int32_t* ps = starts ? (const int32_t*)starts->data_ptr() : nullptr;
+        const int32_t* pi = index ? (const int32_t*)index->data_ptr() : nullptr;
+        void *po = out->data_ptr(), *pw = ws ? ws->data_ptr() : nullptr;
+        const size_t wb = ws ? bytes_of(*ws) : 0;
+        int rc;
+        Py_BEGIN_ALLOW_THREADS
+        rc = otter_hip_linear_forward(h, px, (size_t)x->stride(0), x_rows, pi, ps, rows, (float*)po, pw, wb, stream);
+        Py_END_ALLOW_THREADS
+        if (rc) return raise_status(rc);
+        return result(a[7], *out);
+    } catch (const std::exception& e) {
+        PyErr_SetString(PyExc_RuntimeError, e.what());
+        return nullptr;
+    }
+}
+
 // the current stream as an integer
 PyObject* current_stream(PyObject*, PyObject*) { return PyLong_FromVoidPtr(stream_now()); }
 
@@ -300,7 +485,8 @@ PyObject* set_error(PyObject*, PyObject* type) {
 }
 
 #define FAST(name) {#name, (PyCFunction)(void (*)(void))name, METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(conv_forward), FAST(conv_chain), FAST(conv_block),
+PyMethodDef methods[] = {FAST(conv_forward), FAST(conv_chain), FAST(conv_block), FAST(kv_append), FAST(kv_read), FAST(kv_attend),
+                         FAST(linear_forward),
                          {"current_stream", current_stream, METH_NOARGS, nullptr},
                          {"set_error", set_error, METH_O, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

@@ -344,15 +344,12 @@ class Library:
     def linear(self, **kw):
         return Linear(self, **kw)
 
-    def check_tensor(self, t, dtype, shape, what, rows=False):
-        """A tensor on the library's GPU of that type and shape (None in it: any size), contiguous, with `rows` but for its first stride."""
+    def check_tensor(self, t, dtype, shape, what):
+        """A contiguous tensor of that type and shape (None in it: any size) on the library's GPU."""
         if not isinstance(t, self.torch.Tensor) or t.device != self.device or t.dtype != dtype:
             raise HipError(-2, "%s: a %s tensor on %s expected" % (what, dtype, self.device))
-        if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)):
-            raise HipError(-2, "%s: shape %s expected, not %s" % (what, tuple(shape), tuple(t.shape)))
-        if not (t[0] if rows and t.dim() and t.shape[0] else t).is_contiguous() or (rows and t.stride(0) < 0):
-            raise HipError(-2, "%s: not contiguous" % what)
-        return t
+        if t.dim() != len(shape) or any(n is not None and n != m for n, m in zip(shape, t.shape)) or not t.is_contiguous():
+            raise HipError(-2, "%s: contiguous, of shape %s expected, not %s" % (what, tuple(shape), tuple(t.shape)))
 
     def global_avgpool(self, x, layout, n, c, h, w):
         """otter_hip_global_avgpool: the mean over H*W of an fp32 blob, [n, c]."""
@@ -678,6 +675,7 @@ class KvBatch:
             raise HipError(-2, "kv_batch: negative n_tokens")
         self.starts, self.lengths, self.pages, self.n_tokens = starts, lengths, pages, int(n_tokens)
         self.args = KvBatchArgs(n, self.n_tokens, pages.shape[1], starts.data_ptr(), lengths.data_ptr(), pages.data_ptr())
+        self._bp = C.addressof(self.args)
 
 
 class KvCache:
@@ -692,43 +690,20 @@ class KvCache:
         self.key_scales, self.value_scales = (lib.empty(n_pages * heads, np.float32) for _ in range(2))
         self.args = KvCacheArgs(heads, head_dim, n_pages, *[t.data_ptr() for t in (self.keys, self.values, self.key_scales,
                                                                                     self.value_scales)])
+        self._cp = C.addressof(self.args)  # the struct as the native call path takes it
 
     def append(self, batch, keys, values):
         """otter_hip_kv_append: keys and values [n_tokens, heads, head_dim], contiguous but for the stride between rows."""
-        L, shape = self.L, (batch.n_tokens, self.heads, self.head_dim)
-        for t, what in ((keys, "keys"), (values, "values")):
-            L.check_tensor(t, L.torch.float32, shape, what, rows=True)
-        L._check(L.lib.otter_hip_kv_append(C.byref(self.args), C.byref(batch.args), L.ptr(keys), C.c_size_t(keys.stride(0)), L.ptr(values),
-                                           C.c_size_t(values.stride(0)), L.stream()))
+        self.L.native.kv_append(self._cp, batch._bp, keys, values, self.L.device_index)
 
     def read(self, batch, keys=None, values=None):
         """otter_hip_kv_read: the batch's rows as floats, [n_tokens, heads, head_dim] each. Returns (keys, values)."""
-        L, shape = self.L, (batch.n_tokens, self.heads, self.head_dim)
-        out = [L.empty(int(np.prod(shape)), np.float32).view(shape) if t is None else L.check_tensor(t, L.torch.float32, shape, "out")
-               for t in (keys, values)]
-        L._check(L.lib.otter_hip_kv_read(C.byref(self.args), C.byref(batch.args), L.ptr(out[0]), L.ptr(out[1]), L.stream()))
-        return tuple(out)
-
-    def _desc(self, q_heads, scale, cap, causal, window, slopes):
-        if slopes is not None:
-            self.L.check_tensor(slopes, self.L.torch.float32, (q_heads,), "slopes")
-        return KvAttendDesc(q_heads, self.head_dim ** -0.5 if scale is None else scale, cap, int(causal), window,
-                            None if slopes is None else slopes.data_ptr())
+        return self.L.native.kv_read(self._cp, batch._bp, keys, values, self.L.device_index)
 
     def attend(self, batch, q, scale=None, cap=0.0, causal=True, window=0, slopes=None, out=None, workspace=None):
         """otter_hip_kv_attend: q [n_tokens, q_heads, head_dim], contiguous but for the stride between rows, over the cache.
         scale None: 1 / sqrt(head_dim). Returns out, of q's shape."""
-        L, f32 = self.L, self.L.torch.float32
-        L.check_tensor(q, f32, (batch.n_tokens, None, self.head_dim), "q", rows=True)
-        desc = self._desc(q.shape[1], scale, cap, causal, window, slopes)
-        out = L.torch.empty(q.shape, dtype=f32, device=L.device) if out is None else L.check_tensor(out, f32, q.shape, "out")
-        if workspace is None:
-            need = L.lib.otter_hip_kv_attend_workspace_bytes(C.byref(self.args), C.byref(batch.args), C.byref(desc))
-            workspace = L.empty(need, np.int8) if need else None
-        L._check(L.lib.otter_hip_kv_attend(C.byref(self.args), C.byref(batch.args), C.byref(desc), L.ptr(q), C.c_size_t(q.stride(0)),
-                                           L.ptr(out), L.ptr(workspace) if workspace is not None else None,
-                                           C.c_size_t(0 if workspace is None else workspace.numel() * workspace.element_size()), L.stream()))
-        return out
+        return self.L.native.kv_attend(self._cp, batch._bp, q, scale, cap, causal, window, slopes, out, workspace, self.L.device_index)
 
 
 class Linear:
@@ -747,6 +722,7 @@ class Linear:
         d = LinearDesc(self.experts, self.in_features, self.out_features, int(gated), act, act_p0)
         lib._check(lib.lib.otter_hip_linear_create(C.byref(d), w.ctypes.data_as(C.c_void_p), s.ctypes.data_as(C.c_void_p),
                                                    b.ctypes.data_as(C.c_void_p) if b is not None else None, C.byref(self.h)))
+        self._hp = self.h.value  # the handle as the native call path takes it
 
     def kernel_kind(self, rows):
         """otter_hip_linear_kernel_kind: 0 the launch for few rows, 1 to 3 those for many."""
@@ -757,25 +733,13 @@ class Linear:
     def forward(self, x, starts=None, index=None, out=None, workspace=None):
         """otter_hip_linear_forward: x [x_rows, in_features], contiguous but for the stride between rows; starts [experts + 1] and
         index [rows] int32. Returns y [rows, out_features]."""
-        L, t = self.L, self.L.torch
-        L.check_tensor(x, t.float32, (None, self.in_features), "x", rows=True)
-        rows = x.shape[0] if index is None else L.check_tensor(index, t.int32, (None,), "index").shape[0]
-        if starts is not None:
-            L.check_tensor(starts, t.int32, (self.experts + 1,), "starts")
-        shape = (rows, self.out_features)
-        out = t.empty(shape, dtype=t.float32, device=L.device) if out is None else L.check_tensor(out, t.float32, shape, "out")
-        if workspace is None:
-            workspace = L.empty(L.lib.otter_hip_linear_workspace_bytes(self.h, x.shape[0], rows), np.int8)
-        L._check(L.lib.otter_hip_linear_forward(
-            self.h, L.ptr(x), C.c_size_t(x.stride(0)), x.shape[0], L.ptr(index) if index is not None else None,
-            L.ptr(starts) if starts is not None else None, rows, L.ptr(out), L.ptr(workspace),
-            C.c_size_t(workspace.numel() * workspace.element_size()), L.stream()))
-        return out
+        return self.L.native.linear_forward(self._hp, self.experts, self.in_features, self.out_features, x, starts, index, out, workspace,
+                                            self.L.device_index)
 
     def close(self):
         if self.h:
             self.L.lib.otter_hip_linear_destroy(self.h)
-            self.h = None
+            self.h = self._hp = None
 
     def __del__(self):
         try:

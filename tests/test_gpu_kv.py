@@ -353,7 +353,7 @@ def test_recorded(hip):
     L = hip.lib
     hip._check(L.otter_hip_record_begin(C.byref(stream)))
     a, b = C.byref(s.cache.args), C.byref(s.now[3].args)
-    d = C.byref(s.cache._desc(4, None, 0.0, True, 0, None))
+    d = C.byref(capi.KvAttendDesc(4, 64 ** -0.5, 0.0, 1, 0, None))
     size = C.c_size_t
     hip._check(L.otter_hip_kv_append(a, b, hip.ptr(k), size(64), hip.ptr(v), size(64), stream))
     hip._check(L.otter_hip_kv_read(a, b, hip.ptr(ko), hip.ptr(vo), stream))
