@@ -695,6 +695,8 @@ int otter_hip_linear_forward(const otter_hip_linear_t* handle, const float* x, s
 /* For tests and profiling: which launch otter_hip_linear_forward takes for that many rows: 0 the one for few rows, 1 to 3 those for many,
  * 32 x 64, 64 x 64 and 64 x 128 results a wave. The results are the same, bit for bit. */
 int otter_hip_linear_kernel_kind(const otter_hip_linear_t* handle, int rows);
+/* Tuning / test hook: that launch for any number of rows (-1: the choice is automatic). */
+int otter_hip_linear_set_kernel(otter_hip_linear_t* handle, int kind);
 
 #ifdef __cplusplus
 }

@@ -93,7 +93,7 @@ EXPORTS = ["otter_hip_init", "otter_hip_shutdown", "otter_hip_last_error", "otte
            "otter_hip_record_begin", "otter_hip_record_end", "otter_hip_record_launch", "otter_hip_record_destroy",
            "otter_hip_kv_page_bytes", "otter_hip_kv_append", "otter_hip_kv_read", "otter_hip_kv_attend_workspace_bytes",
            "otter_hip_kv_attend", "otter_hip_linear_create", "otter_hip_linear_destroy", "otter_hip_linear_workspace_bytes",
-           "otter_hip_linear_forward", "otter_hip_linear_kernel_kind"]
+           "otter_hip_linear_forward", "otter_hip_linear_kernel_kind", "otter_hip_linear_set_kernel"]
 
 
 def load_cdll():
@@ -729,6 +729,10 @@ class Linear:
         r = self.L.lib.otter_hip_linear_kernel_kind(self.h, rows)
         self.L._check(min(r, 0))
         return r
+
+    def set_kernel(self, kind):
+        """otter_hip_linear_set_kernel: that launch for any number of rows, -1 the automatic choice."""
+        self.L._check(self.L.lib.otter_hip_linear_set_kernel(self.h, kind))
 
     def forward(self, x, starts=None, index=None, out=None, workspace=None):
         """otter_hip_linear_forward: x [x_rows, in_features], contiguous but for the stride between rows; starts [experts + 1] and

@@ -2480,7 +2480,7 @@ int otter_hip_linear_create(const otter_hip_linear_desc* desc, const int8_t* wei
         otter_hip_linear_destroy(h);
         return rc;
     }
-    h->v = {h->w, h->scale, h->bias, d.experts, d.in_features, d.out_features, tiles, steps, d.gated, d.activation_type, d.activation_param0};
+    h->v = {h->w, h->scale, h->bias, d.experts, d.in_features, d.out_features, tiles, steps, d.gated, d.activation_type, d.activation_param0, -1};
     *handle = h;
     return OTTER_HIP_OK;
 }
@@ -2492,6 +2492,12 @@ size_t otter_hip_linear_workspace_bytes(const otter_hip_linear_t* handle, int x_
 int otter_hip_linear_kernel_kind(const otter_hip_linear_t* handle, int rows) {
     if (!handle || rows < 1) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_kernel_kind: null or no rows");
     return linear_choice(handle->v, rows);
+}
+
+int otter_hip_linear_set_kernel(otter_hip_linear_t* handle, int kind) {
+    if (!handle || kind < -1 || kind > 3) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_set_kernel: null or no such launch");
+    handle->v.force = kind;
+    return OTTER_HIP_OK;
 }
 
 int otter_hip_linear_forward(const otter_hip_linear_t* handle, const float* x, size_t x_stride, int x_rows, const int32_t* index,

@@ -6,6 +6,8 @@
 
 namespace ohip {
 
+typedef float v4f __attribute__((ext_vector_type(4)));
+
 // c * was / s rounded half away from zero, exactly: the product of a code and a float is exact in 64 bits, the comparison with the
 // middle between two codes one fused multiply-add.
 __device__ __forceinline__ int code_again(int c, float was, float s) {
@@ -170,8 +172,10 @@ __device__ __forceinline__ void kv_read_block(const KvView& c, const KvTile& t, 
         for (int r = 0; r < 4; ++r) {
             if (p.token + r < from || p.token + r >= to) continue;
             float* const to_row = rows + (ptrdiff_t)(p.token + r) * (ptrdiff_t)stride + p.dim;
-            if (quads) *reinterpret_cast<float4*>(to_row) = {v[r][0], v[r][1], v[r][2], v[r][3]};
-            else {
+            if (quads) {  // (four times the codes, and seldom read again by the GPU: not kept in the caches. 27 MB of codes 38.5 -> 21.8 us)
+                const v4f f = {v[r][0], v[r][1], v[r][2], v[r][3]};
+                __builtin_nontemporal_store(f, reinterpret_cast<v4f*>(to_row));
+            } else {
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (p.dim + e < c.dim) to_row[e] = v[r][e];

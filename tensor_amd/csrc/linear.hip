@@ -81,6 +81,7 @@ struct LinearArgs {
     const int32_t *index, *starts;
     int x_rows, rows;
     float* y;
+    bool streams;
 };
 
 // Expert and rows of a tile of `unit` rows: [begin, end), empty where the tile is behind its expert's rows.
@@ -126,39 +127,60 @@ __device__ __forceinline__ float4 linear_value(const v4i& acc, float xs, const L
     return {__fmaf_rn((float)acc[0], __fmul_rn(xs, o.scale.x), o.bias.x), __fmaf_rn((float)acc[1], __fmul_rn(xs, o.scale.y), o.bias.y),
             __fmaf_rn((float)acc[2], __fmul_rn(xs, o.scale.z), o.bias.z), __fmaf_rn((float)acc[3], __fmul_rn(xs, o.scale.w), o.bias.w)};
 }
-__device__ __forceinline__ float gate(float g, float up) { return __fmul_rn(__fdiv_rn(g, __fadd_rn(1.f, __expf(-g))), up); }
-// Four consecutive outputs of one row, `column` the first.
-__device__ __forceinline__ void linear_put(const LinearArgs& a, int row, int column, const float4& v) {
-    float* const to = a.y + (size_t)row * a.w.out + column;
-    if (a.w.out % 4 == 0 && ((size_t)a.y & 15) == 0) {
-        if (column < a.w.out) *reinterpret_cast<float4*>(to) = v;
-    } else {
-        if (column < a.w.out) to[0] = v.x;
-        if (column + 1 < a.w.out) to[1] = v.y;
-        if (column + 2 < a.w.out) to[2] = v.z;
-        if (column + 3 < a.w.out) to[3] = v.w;
+// What becomes of a result: an instance each, as 128 results of a lane with a choice in front of each were 24 thousand instructions, and a
+// third of the time of a launch.
+enum { LINEAR_PLAIN, LINEAR_CLAMP, LINEAR_LEAKY, LINEAR_SIGMOID, LINEAR_MISH, LINEAR_GATED };
+static int linear_end(const LinearView& w) {
+    switch (w.gated ? -1 : w.act) {
+    case -1: return LINEAR_GATED;
+    case 1:
+    case 3: return LINEAR_CLAMP;
+    case 2: return LINEAR_LEAKY;
+    case 4: return LINEAR_SIGMOID;
+    case 5: return LINEAR_MISH;
+    default: return LINEAR_PLAIN;
     }
 }
-template <bool GATED>
+template <int END>
+__device__ __forceinline__ float linear_act(float v, float up, float p0) {
+    if constexpr (END == LINEAR_CLAMP) return fminf(fmaxf(v, 0.f), p0);  // (p0: 6 or infinity)
+    if constexpr (END == LINEAR_LEAKY) return activate(v, 2, p0);
+    if constexpr (END == LINEAR_SIGMOID) return activate(v, 4, p0);
+    if constexpr (END == LINEAR_MISH) return activate(v, 5, p0);
+    if constexpr (END == LINEAR_GATED) return __fmul_rn(__fdiv_rn(v, __fadd_rn(1.f, __expf(-v))), up);
+    return v;
+}
+typedef float v4f __attribute__((ext_vector_type(4)));
+// Four consecutive outputs of one row, `column` the first. Results beyond what the L2s hold (a.streams) are not kept there.
+template <int END>
 __device__ __forceinline__ void linear_store(const LinearArgs& a, int row, float xs, int n_tile, const v4i& acc, const v4i& acc_up, const LinearOut& o,
-                                             const LinearOut& o_up) {
-    float4 v = linear_value(acc, xs, o);
-    if constexpr (GATED) {
-        const float4 u = linear_value(acc_up, xs, o_up);
-        v = {gate(v.x, u.x), gate(v.y, u.y), gate(v.z, u.z), gate(v.w, u.w)};
-    } else if (a.w.act) {
-        v = {activate(v.x, a.w.act, a.w.act_p0), activate(v.y, a.w.act, a.w.act_p0), activate(v.z, a.w.act, a.w.act_p0), activate(v.w, a.w.act, a.w.act_p0)};
+                                             const LinearOut& o_up, bool quads) {
+    const float4 v = linear_value(acc, xs, o);
+    float4 u = {0.f, 0.f, 0.f, 0.f};
+    if constexpr (END == LINEAR_GATED) u = linear_value(acc_up, xs, o_up);
+    const v4f r = {linear_act<END>(v.x, u.x, a.w.act_p0), linear_act<END>(v.y, u.y, a.w.act_p0), linear_act<END>(v.z, u.z, a.w.act_p0),
+                   linear_act<END>(v.w, u.w, a.w.act_p0)};
+    const int column = n_tile * 16 + (int)((threadIdx.x >> 4) & 3) * 4;
+    float* const to = a.y + (size_t)row * a.w.out + column;
+    if (quads) {
+        if (column >= a.w.out) return;
+        if (a.streams) __builtin_nontemporal_store(r, reinterpret_cast<v4f*>(to));
+        else *reinterpret_cast<v4f*>(to) = r;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (column + e < a.w.out) to[e] = r[e];
     }
-    linear_put(a, row, n_tile * 16 + (int)((threadIdx.x >> 4) & 3) * 4, v);
 }
+__device__ __forceinline__ bool linear_quads(const LinearArgs& a) { return a.w.out % 4 == 0 && ((size_t)a.y & 15) == 0; }
 
 // 16 outputs (gated: 16 of either half) x 16 rows a workgroup, the inputs dealt to its W waves, whose sums meet in LDS. Both operands
 // come straight from memory in lane order, several steps of them asked for before the first is used; this is the launch for few rows,
 // where reading the weights is the work. (32 and 64 rows a workgroup, which read the weights less often, were the fastest of all launches
 // for no size.)
-template <bool GATED, int W>
+template <int END, int W>
 __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
-    constexpr int G = GATED ? 2 : 1, AHEAD = 4;
+    constexpr int G = END == LINEAR_GATED ? 2 : 1, AHEAD = 4;
     __shared__ v4i sums[W][G][64];
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const unsigned n_tiles = (unsigned)a.w.tiles / G;
@@ -198,14 +220,14 @@ __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
 #pragma unroll
         for (int n = 0; n < W; ++n) sum[h] += sums[n][h][lane];
     const LinearOut o = linear_out(a, t.expert, n_tile * G), o_up = linear_out(a, t.expert, n_tile * G + G - 1);
-    linear_store<GATED>(a, row, src < 0 ? 0.f : a.scale[src], n_tile, sum[0], sum[1], o, o_up);
+    linear_store<END>(a, row, src < 0 ? 0.f : a.scale[src], n_tile, sum[0], sum[1], o, o_up, linear_quads(a));
 }
 
 // 64 NT outputs x 16 RT rows a workgroup, 16 NT outputs a wave: the launch for many rows. A wave loads its weights, which no other
 // wave of the workgroup reads, straight into registers, a stage of 128 inputs ahead; the rows' codes, which all four waves read, go
 // through LDS, in lane order too (a 16-byte piece of a row is a lane's). A stage is 8 NT RT matrix instructions a wave against 2 RT KB
 // from LDS and 2 NT KB from memory: with 4 and 8 that is 64 and 32 bytes a cycle of a compute unit's 128 and 64.
-template <int NT, int RT, bool GATED>
+template <int NT, int RT, int END>
 __global__ void __launch_bounds__(256, 2) linear_many_kernel(LinearArgs a) {
     constexpr int MINE = RT / 4;  // tiles of 16 rows that a wave brings in
     __shared__ v4i rows[3][RT][2][64];
@@ -284,42 +306,62 @@ __global__ void __launch_bounds__(256, 2) linear_many_kernel(LinearArgs a) {
         stage(std::integral_constant<int, 1>{}, s + 2);
     }
     if (s < even) stage(std::integral_constant<int, 0>{}, s);
-    constexpr int G = GATED ? 2 : 1;
+    constexpr int G = END == LINEAR_GATED ? 2 : 1;
+    float xs[RT];
 #pragma unroll
-    for (int n = 0; n < NT; n += G) {
-        if (tile0 + n >= a.w.tiles) break;
-        const LinearOut o = linear_out(a, t.expert, tile0 + n), o_up = linear_out(a, t.expert, tile0 + n + G - 1);
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-            const int row = t.begin + r * 16 + (lane & 15);
-            if (row >= t.end) continue;
-            const int src = linear_source(a, row);
-            linear_store<GATED>(a, row, src < 0 ? 0.f : a.scale[src], (tile0 + n) / G, acc[n][r], acc[n + G - 1][r], o, o_up);
-        }
+    for (int r = 0; r < RT; ++r) {
+        const int src = linear_source(a, min(t.begin + r * 16 + (lane & 15), t.end - 1));
+        xs[r] = src < 0 ? 0.f : a.scale[src];
     }
+    const auto finish = [&](bool quads) {
+#pragma unroll
+        for (int n = 0; n < NT; n += G) {
+            if (tile0 + n >= a.w.tiles) break;
+            const LinearOut o = linear_out(a, t.expert, tile0 + n), o_up = linear_out(a, t.expert, tile0 + n + G - 1);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const int row = t.begin + r * 16 + (lane & 15);
+                if (row < t.end) linear_store<END>(a, row, xs[r], (tile0 + n) / G, acc[n][r], acc[n + G - 1][r], o, o_up, quads);
+            }
+        }
+    };
+    if (linear_quads(a)) finish(true);
+    else finish(false);
 }
 
+#define OHIP_LINEAR_END(CALL)                                  \
+    switch (linear_end(a.w)) {                                 \
+    case LINEAR_GATED: CALL(LINEAR_GATED); break;              \
+    case LINEAR_CLAMP: CALL(LINEAR_CLAMP); break;              \
+    case LINEAR_LEAKY: CALL(LINEAR_LEAKY); break;              \
+    case LINEAR_SIGMOID: CALL(LINEAR_SIGMOID); break;          \
+    case LINEAR_MISH: CALL(LINEAR_MISH); break;                \
+    default: CALL(LINEAR_PLAIN); break;                        \
+    }
 template <int W>
 static void launch_few(const LinearArgs& a, const LinearRows& r, hipStream_t stream) {
     const dim3 grid((unsigned)(a.w.tiles / (a.w.gated ? 2 : 1)) * (unsigned)linear_row_tiles(a.w, r, 16));
-    if (a.w.gated) launch(linear_few_kernel<true, W>, grid, dim3(64 * W), 0, stream, a);
-    else launch(linear_few_kernel<false, W>, grid, dim3(64 * W), 0, stream, a);
+#define CALL(END) launch(linear_few_kernel<END, W>, grid, dim3(64 * W), 0, stream, a)
+    OHIP_LINEAR_END(CALL)
+#undef CALL
 }
 
 template <int NT, int RT>
 static void launch_many(const LinearArgs& a, const LinearRows& r, hipStream_t stream) {
     const dim3 grid((unsigned)((a.w.tiles + 4 * NT - 1) / (4 * NT)) * (unsigned)linear_row_tiles(a.w, r, 16 * RT));
-    if (a.w.gated) launch(linear_many_kernel<NT, RT, true>, grid, dim3(256), 0, stream, a);
-    else launch(linear_many_kernel<NT, RT, false>, grid, dim3(256), 0, stream, a);
+#define CALL(END) launch(linear_many_kernel<NT, RT, END>, grid, dim3(256), 0, stream, a)
+    OHIP_LINEAR_END(CALL)
+#undef CALL
 }
 
-// The launch that is the fastest by a model of the measured ones (3 to 128 steps of inputs, 512 to 8192 outputs, 1 to 16384 rows, 1 to
-// 64 experts; microseconds without the codes). The one for few rows reads weights and rows from the caches at 10 TB/s, 16 x 16 results
-// at a time, but waits 1.2 for every four steps of a wave. The others take `each` for a stage of a workgroup by itself and `busy` where
-// every compute unit has one, n times that for n: 64 x 64 results a wave are the least traffic, 32 x 64 start the soonest. Against
-// the fastest of the five: 4096 x 4096 weights, 128 rows 23.1 us (few: 26.1), 512 rows 27.3 (64 x 64 a wave: 35.0), 2048 rows 61.9 (32
-// x 64: 73.7), 8192 rows 196 (64 x 64: 214).
+// The launch that is the fastest by a model fitted to 92 measured products (16 to 128 steps of inputs, 512 to 8192 outputs, 1 to 16384
+// rows, 1 to 64 experts; microseconds without the codes): 1 % over the fastest of the four on the mean, 18 % at most. The one for few rows
+// reads weights and rows from the caches at 8 TB/s, 16 x 16 results at a time, but waits 1.2 for every 32 steps. The others take `each`
+// for a stage of a workgroup by itself and `busy` where every compute unit has one, n times that for n: 64 x 128 results a wave are
+// the least traffic, 32 x 64 start the soonest. 4096 x 4096 weights with codes: 128 rows 22 us (few: 26), 512 rows 26.0 (64 x 64: 30.6),
+// 2048 rows 56.2 (32 x 64: 72.6), 8192 rows 193 (64 x 64: 216).
 int linear_choice(const LinearView& w, int rows) {
+    if (w.force >= 0) return w.force;
     const auto row_tiles = [&](int unit) {
         return w.experts == 1 ? (rows + unit - 1) / unit : rows / unit + (rows < w.experts ? rows : w.experts) * 0.5;
     };
@@ -328,8 +370,8 @@ int linear_choice(const LinearView& w, int rows) {
         const double load = (w.tiles + 4 * nt - 1) / (4 * nt) * row_tiles(16 * rt) / 256 * busy;
         return start + stages * (load > each ? load : each);
     };
-    const double waits = ((w.steps + 31) / 32) * 1.2, reads = row_tiles(16) * 2 * weights / 10e6;
-    const double t[4] = {2.5 + (waits > reads ? waits : reads), many(2, 4, 5, 0.5, 0.48), many(4, 4, 7, 0.8, 0.69), many(4, 8, 9, 1.65, 1.2)};
+    const double waits = ((w.steps + 31) / 32) * 1.2, reads = row_tiles(16) * 2 * weights / 8e6;
+    const double t[4] = {2.7 + (waits > reads ? waits : reads), many(2, 4, 4.4, 0.62, 0.61), many(4, 4, 3.2, 1.1, 0.89), many(4, 8, 10, 1.55, 1.3)};
     int best = 0;
     for (int i = 1; i < 4; ++i)
         if (t[i] < t[best]) best = i;
@@ -341,7 +383,9 @@ hipError_t run_linear(const LinearView& w, const LinearRows& r, void* workspace,
     launch(linear_codes_kernel, dim3((unsigned)r.x_rows), dim3(256), 0, stream, r.x, r.x_stride, w.in, (int)linear_row_bytes(w.steps), c.scale, c.codes);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    const LinearArgs a{w, c.scale, c.codes, r.index, r.starts, r.x_rows, r.rows, r.y};
+    LinearArgs a{w, c.scale, c.codes, r.index, r.starts, r.x_rows, r.rows, r.y, (size_t)r.rows * w.out * 4 > ((size_t)32 << 20)};
+    if (w.act == 1) a.w.act_p0 = __builtin_inff();
+    if (w.act == 3) a.w.act_p0 = 6.f;
     switch (linear_choice(w, r.rows)) {
     case 0: {
         // eight waves share the inputs where the workgroups alone would leave compute units without work

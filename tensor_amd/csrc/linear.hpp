@@ -12,6 +12,7 @@ struct LinearView {
     int tiles, steps;
     int gated, act;
     float act_p0;
+    int force;  // the launch that otter_hip_linear_set_kernel names, or -1
 };
 struct LinearRows {
     const float* x;

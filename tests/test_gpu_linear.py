@@ -130,35 +130,48 @@ def test_a_row_is_the_same_whatever_stands_beside_it(hip):
         assert hip.torch.equal(whole[a:e], layer.forward(x[a:e]))
 
 
-@pytest.mark.parametrize("kind,experts,k,n,rows,gated", [
-    (1, 1, 1000, 1030, 1500, False), (1, 5, 260, 501, 3000, False), (1, 4, 448, 640, 900, True), (1, 3, 64, 520, 16000, False),
-    (2, 1, 1000, 1030, 9000, False), (2, 3, 320, 1900, 9001, False), (2, 2, 130, 1500, 9000, True), (2, 1, 64, 4200, 9000, False),
-    (3, 1, 1090, 4100, 4100, False), (3, 2, 576, 3900, 5000, False), (3, 3, 500, 1990, 6000, True), (3, 1, 64, 8200, 16000, False)])
-def test_launches_for_many_rows(hip, kind, experts, k, n, rows, gated):
-    """Every row of each of the launches for many rows, against the launch for few rows, 16 at a time of one expert, bit for bit; that
-    one is compared with the model above, and here at the first and the last of its rows."""
+@pytest.mark.parametrize("kind", [0, 1, 2, 3])
+@pytest.mark.parametrize("k,n", [(64, 16), (65, 130), (128, 256), (130, 33), (200, 515), (448, 64), (577, 300), (1000, 270)])
+def test_every_launch(hip, kind, k, n):
+    """Each launch at sizes that the choice would not give it: outputs and rows that end inside its tiles, steps of inputs in odd and even
+    numbers, experts with none, one and many rows, a gate, every activation."""
+    rng = np.random.default_rng(kind + k)
+    for counts, gated, act in (([1], False, 0), ([300], False, 1), ([0, 130, 0, 129, 1], False, 0), ([70, 0, 65], True, 0), ([128], False, 2),
+                               ([257], False, 3), ([40], False, 4), ([33, 31], False, 5), ([64], True, 0)):
+        e = len(counts)
+        starts, index = route(rng, e, counts, 50, front=2, behind=1)
+        x = rng.normal(0, 1, (50, k)).astype(np.float32)
+        w, s, b = weights(rng, e, 2 * n if gated else n, k)
+        layer = hip.linear(weight=w, scale=s, bias=b, gated=gated, act=act, act_p0=0.1)
+        layer.set_kernel(kind)
+        assert layer.kernel_kind(5) == kind
+        into = rng.normal(0, 1, (len(index), n)).astype(np.float32)
+        out = layer.forward(hip.to_device(x), dev(hip, starts), dev(hip, index), out=hip.to_device(into))
+        check_close(out.cpu().numpy(), *linear(x, w, s, b, into, starts=starts, index=index, gated=gated, act=act, act_p0=0.1))
+        layer.close()
+
+
+@pytest.mark.parametrize("experts,k,n,rows,gated", [(1, 1000, 1030, 1500, False), (4, 448, 640, 900, True), (3, 320, 1900, 9001, False),
+                                                    (2, 130, 1500, 9000, True), (1, 1090, 4100, 4100, False), (1, 64, 8200, 16000, False)])
+def test_launches_give_the_same_bits(hip, experts, k, n, rows, gated):
+    """Many rows, among them results that are too many for the caches: every launch as the automatic one, bit for bit."""
     torch = hip.torch
-    rng = np.random.default_rng(kind * rows)
+    rng = np.random.default_rng(rows)
     w, s, b = weights(rng, experts, 2 * n if gated else n, k)
     layer = hip.linear(weight=w, scale=s, bias=b, gated=gated)
-    assert layer.kernel_kind(rows) == kind and layer.kernel_kind(16) == 0
+    assert layer.kernel_kind(rows) > 0 and layer.kernel_kind(16) == 0
     cuts = np.sort(rng.integers(0, rows + 1, experts - 1))
-    starts = np.concatenate([[3], np.maximum(cuts, 3), [rows]]).astype(np.int32)
+    starts = dev(hip, np.concatenate([[3], np.maximum(cuts, 3), [rows]]))
     x = hip.to_device(rng.normal(0, 1, (rows // 2, k)).astype(np.float32))
-    index = rng.integers(0, rows // 2, rows).astype(np.int32)
-    out = layer.forward(x, dev(hip, starts), dev(hip, index), out=torch.full((rows, n), 5.0, device=hip.device))
-    assert (out[:3] == 5).all()
-    for e in range(experts):
-        one = hip.linear(weight=w[e], scale=s[e], bias=b[e], gated=gated)
-        for a in [*range(int(starts[e]), int(starts[e + 1]), 16)]:
-            z = min(a + 16, int(starts[e + 1]))
-            i = dev(hip, index[a:z])
-            assert torch.equal(out[a:z], one.forward(x, index=i)), (e, a)
-        one.close()
-    for r in (3, rows - 1):
-        e = int(np.searchsorted(starts, r, side="right")) - 1
-        xn = x[int(index[r])].cpu().numpy()[None]
-        check_close(out[r:r + 1].cpu().numpy(), *linear(xn, w[e:e + 1], s[e:e + 1], b[e:e + 1], np.zeros((1, n), np.float32), gated=gated))
+    index = dev(hip, rng.integers(0, rows // 2, rows))
+    want = layer.forward(x, starts, index, out=torch.full((rows, n), 5.0, device=hip.device))
+    assert (want[:3] == 5).all() and not (want[3:] == 5).any(1).all()
+    for kind in range(4):
+        layer.set_kernel(kind)
+        assert torch.equal(want, layer.forward(x, starts, index, out=torch.full((rows, n), 5.0, device=hip.device)))
+    layer.set_kernel(-1)
+    with pytest.raises(capi.HipError):
+        layer.set_kernel(4)
     layer.close()
 
 

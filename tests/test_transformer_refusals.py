@@ -102,5 +102,5 @@ def test_layers_without_a_part(lib):
     assert lib.otter_hip_linear_create(C.byref(d), v, v, None, None) == -2
     assert lib.otter_hip_linear_forward(None, v, C.c_size_t(64), 1, None, None, 1, v, v, C.c_size_t(1 << 20), None) == -2
     assert lib.otter_hip_linear_workspace_bytes(None, 1, 1) == 0
-    assert lib.otter_hip_linear_kernel_kind(None, 1) == -2
+    assert lib.otter_hip_linear_kernel_kind(None, 1) == -2 and lib.otter_hip_linear_set_kernel(None, 0) == -2
     assert lib.otter_hip_linear_destroy(None) == 0
