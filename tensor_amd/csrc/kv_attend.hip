@@ -354,9 +354,8 @@ __global__ void __launch_bounds__(256, (kv_waves<KC, EXTRA>(STAGED))) kv_attend_
     const unsigned lane16 = (unsigned)lane * 16u;
     const int head = (int)(blockIdx.x % (unsigned)a.c.heads);
     const int tile = a.tiles - 1 - (int)(blockIdx.x / (unsigned)a.c.heads);  // (a causal prompt's last tiles have the most to read)
-    const int i = kv_find(a.b.starts, a.b.n_seqs, a.b.n_tokens, a.group, 64, 1, tile);
-    const KvSeq s = kv_sequence(a.b, i);
-    const int row0 = (tile - kv_tile_base(a.b.starts, i, a.b.n_tokens, a.group, 64, 1)) * 64, rows = s.count * a.group;
+    const KvSeq s = kv_locate<true>(a.b.starts, a.b.lengths, a.b.n_seqs, a.b.n_tokens, a.group, 64, 1, tile);
+    const int row0 = s.tile * 64, rows = s.count * a.group;
     if (row0 < 0 || row0 >= rows) return;
     const int tiles = (min(rows - row0, 64) + 15) >> 4;      // of 16 rows
     const int shares = tiles == 1 ? 4 : tiles == 2 ? 2 : 1;  // waves that share a tile's pages
@@ -383,7 +382,7 @@ __global__ void __launch_bounds__(256, (kv_waves<KC, EXTRA>(STAGED))) kv_attend_
 #pragma unroll
         for (int e = 0; e < 4; ++e) run.o[dt][e] = 0.f;
     PageWalk walk;
-    walk.table = a.b.pages + (size_t)i * a.b.max_pages;
+    walk.table = a.b.pages + (size_t)s.index * a.b.max_pages;
     // pages [begin, end) of positions [lo, hi), the part-th of `parts` equal shares
     const auto deal = [&](int lo, int hi, int part, int parts) {
         const int page0 = lo / KV_BLOCK, pages = max((hi + KV_BLOCK - 1) / KV_BLOCK - page0, 0), each = (pages + parts - 1) / parts;

@@ -29,15 +29,14 @@ struct KvTile {
 };
 // tile -> (sequence, block)
 __device__ __forceinline__ KvTile kv_block_of(const KvBatch& b, int n_pages, int tile) {
-    const int i = kv_find(b.starts, b.n_seqs, b.n_tokens, 1, KV_BLOCK, 2, tile);
     KvTile t;
-    t.seq = kv_sequence(b, i);
-    const int block = (t.seq.first >> 6) + (tile - kv_tile_base(b.starts, i, b.n_tokens, 1, KV_BLOCK, 2));
-    t.any = tile >= kv_tile_base(b.starts, i, b.n_tokens, 1, KV_BLOCK, 2) && t.seq.count > 0 && block <= ((t.seq.length - 1) >> 6);
+    t.seq = kv_locate<true>(b.starts, b.lengths, b.n_seqs, b.n_tokens, 1, KV_BLOCK, 2, tile);
+    const int block = (t.seq.first >> 6) + t.seq.tile;
+    t.any = t.seq.tile >= 0 && t.seq.count > 0 && block <= ((t.seq.length - 1) >> 6);
     t.position = block * KV_BLOCK;
     t.page = -1;
     if (t.any && block >= 0 && block < b.max_pages) {
-        const int page = b.pages[(size_t)i * b.max_pages + block];
+        const int page = b.pages[(size_t)t.seq.index * b.max_pages + block];
         if ((unsigned)page < (unsigned)n_pages) t.page = page;
     }
     return t;

@@ -39,36 +39,44 @@ struct KvBatch {
 
 // One sequence of a batch as the kernels see it: what a table that is wrong could say is cut to what the buffers hold.
 struct KvSeq {
+    int index;
     int begin, count;  // its rows
     int length;        // tokens, with those of the rows
     int first;         // position of its first row (below 0: the batch says more rows than tokens)
+    int tile;          // of the sequence (below 0: of none)
 };
-__device__ __forceinline__ KvSeq kv_sequence(const KvBatch& b, int i) {
-    KvSeq s;
-    s.begin = min(max(b.starts[i], 0), b.n_tokens);
-    s.count = min(max(b.starts[i + 1], s.begin), b.n_tokens) - s.begin;
-    s.length = max(b.lengths[i], 0);
-    s.first = s.length - s.count;
-    return s;
-}
 
 // Work is dealt to tiles of `unit` rows of a sequence without a list of them: sequence i's tiles begin at starts[i] * mul / unit +
 // slack * i, which leaves each at least as many as it needs (ceil(n / unit) <= floor difference + 1, and one more where a tile is
-// aligned to positions, not to rows). The largest i whose tiles begin at or before `tile`, by the lanes of a wave: a load for each 64-fold.
-__device__ __forceinline__ int kv_tile_base(const int32_t* starts, int i, int limit, int mul, int unit, int slack) {
-    return (int)((unsigned)(min(max(starts[i], 0), limit) * mul) / (unsigned)unit) + slack * i;
+// aligned to positions, not to rows). The largest i whose tiles begin at or before `tile`, by the lanes of a wave: a load for each
+// 64-fold of sequences, and what is to be known of the one that is found comes with the last of them.
+__device__ __forceinline__ int kv_tile_base(int start, int i, int limit, int mul, int unit, int slack) {
+    return (int)((unsigned)(min(max(start, 0), limit) * mul) / (unsigned)unit) + slack * i;
 }
-__device__ __forceinline__ int kv_find(const int32_t* starts, int n, int limit, int mul, int unit, int slack, int tile) {
+template <bool LENGTHS>
+__device__ __forceinline__ KvSeq kv_locate(const int32_t* starts, const int32_t* lengths, int n, int limit, int mul, int unit, int slack, int tile) {
     const int lane = (int)(threadIdx.x & 63);
     int lo = 0;
-    while (n > 1) {
-        const int step = (n + 63) >> 6, i = lane * step;
-        const bool before = i < n && kv_tile_base(starts, lo + min(i, n - 1), limit, mul, unit, slack) <= tile;
-        const int k = max(__popcll(__ballot(before)), 1) - 1;
+    for (;;) {
+        const int step = (n + 63) >> 6, i = lane * step, at = lo + min(i, n - 1);
+        const int from = starts[at], to = starts[at + 1];
+        int length = 0;
+        if constexpr (LENGTHS) length = lengths[at];
+        const int base = kv_tile_base(from, at, limit, mul, unit, slack);
+        const int k = max(__popcll(__ballot(i < n && base <= tile)), 1) - 1;
+        if (step == 1) {
+            KvSeq s;
+            s.index = __builtin_amdgcn_readfirstlane(lo + k);
+            s.begin = min(max(__builtin_amdgcn_readlane(from, k), 0), limit);
+            s.count = min(max(__builtin_amdgcn_readlane(to, k), s.begin), limit) - s.begin;
+            s.length = max(__builtin_amdgcn_readlane(length, k), 0);
+            s.first = s.length - s.count;
+            s.tile = tile - __builtin_amdgcn_readlane(base, k);
+            return s;
+        }
         lo += k * step;
         n = min(step, n - k * step);
     }
-    return __builtin_amdgcn_readfirstlane(lo);
 }
 
 // |x| of a finite value, 0 for an infinity or NaN: what a scale is found from.

@@ -94,10 +94,10 @@ __device__ __forceinline__ LinearTile linear_tile(const LinearArgs& a, int tile,
         t.expert = 0, t.begin = tile * unit, t.end = min(t.begin + unit, a.rows);
         return t;
     }
-    t.expert = kv_find(a.starts, a.w.experts, a.rows, 1, unit, 1, tile);
-    const int from = min(max(a.starts[t.expert], 0), a.rows), to = min(max(a.starts[t.expert + 1], from), a.rows);
-    const int n = tile - kv_tile_base(a.starts, t.expert, a.rows, 1, unit, 1);
-    t.begin = n < 0 ? to : min(from + n * unit, to);
+    const KvSeq s = kv_locate<false>(a.starts, nullptr, a.w.experts, a.rows, 1, unit, 1, tile);
+    t.expert = s.index;
+    const int to = s.begin + s.count;
+    t.begin = s.tile < 0 ? to : min(s.begin + s.tile * unit, to);
     t.end = min(t.begin + unit, to);
     return t;
 }
