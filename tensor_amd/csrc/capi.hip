@@ -2333,6 +2333,9 @@ size_t otter_hip_kv_page_bytes(int heads, int head_dim) {
     return heads < 1 || head_dim < 1 || head_dim > 256 ? 0 : (size_t)heads * ((head_dim + 63) / 64) * 4096;
 }
 
+// A launch has fewer than 2^32 work-items: workgroups of 256, and of 512.
+constexpr size_t kMostGroups = 1u << 24, kMostLargeGroups = 1u << 23;
+
 // Both structs checked, and turned into what the launches take. The limits keep tiles, rows and positions in 32 bits.
 static int kv_arguments(const char* who, const otter_hip_kv_cache* cache, const otter_hip_kv_batch* batch, KvView* c, KvBatch* b) {
     const std::string name(who);
@@ -2343,7 +2346,7 @@ static int kv_arguments(const char* who, const otter_hip_kv_cache* cache, const 
     if (((size_t)cache->keys | (size_t)cache->values) & 15) return fail(OTTER_HIP_ERR_INVALID, name + ": keys and values must be 16-byte aligned");
     if (batch->n_seqs < 0 || batch->n_tokens < 0 || batch->max_pages < 0) return fail(OTTER_HIP_ERR_INVALID, name + ": negative size");
     if (batch->n_seqs > (1 << 20) || batch->max_pages > (1 << 24) || (size_t)batch->n_tokens * cache->heads * cache->head_dim >= (1ull << 40) ||
-        ((size_t)batch->n_tokens / KV_BLOCK + 2 * (size_t)batch->n_seqs) * 2 * cache->heads >= (1ull << 31))
+        ((size_t)batch->n_tokens / KV_BLOCK + 2 * (size_t)batch->n_seqs) * 2 * cache->heads >= kMostGroups)
         return fail(OTTER_HIP_ERR_UNSUPPORTED, name + ": batch too large");
     if (batch->n_seqs > 0 && (!batch->starts || !batch->lengths || (batch->max_pages > 0 && !batch->pages)))
         return fail(OTTER_HIP_ERR_INVALID, name + ": null");
@@ -2378,11 +2381,12 @@ static int kv_attend_arguments(const char* who, const otter_hip_kv_cache* cache,
     if (int rc = kv_arguments(who, cache, batch, c, b)) return rc;
     if (!d) return fail(OTTER_HIP_ERR_INVALID, name + ": null");
     if (d->q_heads < 1 || d->q_heads % c->heads) return fail(OTTER_HIP_ERR_INVALID, name + ": q_heads must be a multiple of heads");
-    if (!std::isfinite(d->scale) || !std::isfinite(d->cap) || d->cap < 0 || (d->cap > 0 && !std::isfinite(d->scale / d->cap)))
+    // (both also in units of log 2, as the launch takes them)
+    if (!std::isfinite(d->scale * 1.5f) || !std::isfinite(d->cap * 1.5f) || d->cap < 0 || (d->cap > 0 && !std::isfinite(d->scale / d->cap)))
         return fail(OTTER_HIP_ERR_INVALID, name + ": scale must be finite, cap 0 or positive");
     if (d->window < 0) return fail(OTTER_HIP_ERR_INVALID, name + ": negative window");
     const size_t group = (size_t)(d->q_heads / c->heads), tiles = (size_t)b->n_tokens * group / 64 + b->n_seqs;
-    if ((size_t)b->n_tokens * d->q_heads >= (1ull << 31) || tiles * c->heads >= (1ull << 31)) return fail(OTTER_HIP_ERR_UNSUPPORTED, name + ": batch too large");
+    if ((size_t)b->n_tokens * d->q_heads >= (1ull << 31) || tiles * c->heads >= kMostGroups) return fail(OTTER_HIP_ERR_UNSUPPORTED, name + ": batch too large");
     *splits = 1, *bytes = 0;
     if (b->n_seqs == 0 || b->n_tokens == 0) return OTTER_HIP_OK;
     *splits = kv_attend_splits((int)tiles, c->heads, b->max_pages);
@@ -2508,12 +2512,13 @@ int otter_hip_linear_forward(const otter_hip_linear_t* handle, const float* x, s
     if (!index && rows > x_rows) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_forward: more rows than x has");
     if (rows == 0) return OTTER_HIP_OK;
     if (!x || !y || x_rows == 0) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_forward: null");
-    if (((size_t)rows / 16 + handle->v.experts + 1) * (size_t)handle->v.tiles >= (1ull << 31))
+    const LinearRows r{x, x_stride, x_rows, index, starts, rows, y};
+    if ((size_t)x_rows >= kMostGroups || linear_groups(handle->v, r) >= kMostLargeGroups)
         return fail(OTTER_HIP_ERR_UNSUPPORTED, "otter_hip_linear_forward: too many rows");
     if (!workspace || workspace_bytes < linear_workspace_bytes(handle->v, x_rows))
         return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_forward: workspace too small");
     if ((size_t)workspace & 15) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_forward: the workspace must be 16-byte aligned");
-    OHIP_CHECK(run_linear(handle->v, {x, x_stride, x_rows, index, starts, rows, y}, workspace, (hipStream_t)stream));
+    OHIP_CHECK(run_linear(handle->v, r, workspace, (hipStream_t)stream));
     return OTTER_HIP_OK;
 }
 

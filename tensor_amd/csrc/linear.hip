@@ -102,7 +102,7 @@ __device__ __forceinline__ LinearTile linear_tile(const LinearArgs& a, int tile,
     return t;
 }
 static int linear_row_tiles(const LinearView& w, const LinearRows& r, int unit) {
-    return r.starts ? r.rows / unit + w.experts : (r.rows + unit - 1) / unit;
+    return r.starts ? r.rows / unit + w.experts : (int)(((size_t)r.rows + unit - 1) / unit);
 }
 
 // Row of x behind a sorted row (an index outside of x: -1).
@@ -338,9 +338,18 @@ __global__ void __launch_bounds__(256, 2) linear_many_kernel(LinearArgs a) {
     case LINEAR_MISH: CALL(LINEAR_MISH); break;                \
     default: CALL(LINEAR_PLAIN); break;                        \
     }
+static size_t few_groups(const LinearView& w, const LinearRows& r) { return (size_t)(w.tiles / (w.gated ? 2 : 1)) * linear_row_tiles(w, r, 16); }
+static size_t many_groups(const LinearView& w, const LinearRows& r, int nt, int rt) {
+    return (size_t)((w.tiles + 4 * nt - 1) / (4 * nt)) * linear_row_tiles(w, r, 16 * rt);
+}
+size_t linear_groups(const LinearView& w, const LinearRows& r) {
+    const int k = linear_choice(w, r.rows);
+    return k == 0 ? few_groups(w, r) : k == 1 ? many_groups(w, r, 2, 4) : k == 2 ? many_groups(w, r, 4, 4) : many_groups(w, r, 4, 8);
+}
+
 template <int W>
 static void launch_few(const LinearArgs& a, const LinearRows& r, hipStream_t stream) {
-    const dim3 grid((unsigned)(a.w.tiles / (a.w.gated ? 2 : 1)) * (unsigned)linear_row_tiles(a.w, r, 16));
+    const dim3 grid((unsigned)few_groups(a.w, r));
 #define CALL(END) launch(linear_few_kernel<END, W>, grid, dim3(64 * W), 0, stream, a)
     OHIP_LINEAR_END(CALL)
 #undef CALL
@@ -348,7 +357,7 @@ static void launch_few(const LinearArgs& a, const LinearRows& r, hipStream_t str
 
 template <int NT, int RT>
 static void launch_many(const LinearArgs& a, const LinearRows& r, hipStream_t stream) {
-    const dim3 grid((unsigned)((a.w.tiles + 4 * NT - 1) / (4 * NT)) * (unsigned)linear_row_tiles(a.w, r, 16 * RT));
+    const dim3 grid((unsigned)many_groups(a.w, r, NT, RT));
 #define CALL(END) launch(linear_many_kernel<NT, RT, END>, grid, dim3(256), 0, stream, a)
     OHIP_LINEAR_END(CALL)
 #undef CALL

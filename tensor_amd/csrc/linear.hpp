@@ -24,6 +24,7 @@ struct LinearRows {
 };
 size_t linear_workspace_bytes(const LinearView& w, int x_rows);
 int linear_choice(const LinearView& w, int rows);  // otter_hip_linear_kernel_kind
+size_t linear_groups(const LinearView& w, const LinearRows& r);  // workgroups of its launch
 hipError_t run_linear(const LinearView& w, const LinearRows& r, void* workspace, hipStream_t stream);
 
 }  // namespace ohip

@@ -45,7 +45,7 @@ def test_caches(lib, kw):
 
 
 @pytest.mark.parametrize("kw", [dict(n_seqs=-1), dict(n_tokens=-1), dict(max_pages=-1), dict(starts=None), dict(lengths=None), dict(pages=None),
-                                dict(n_seqs=1 << 21), dict(max_pages=1 << 25), dict(n_seqs=1 << 20, heads=4096),
+                                dict(n_seqs=1 << 21), dict(max_pages=1 << 25), dict(n_seqs=1 << 20, heads=4096), dict(n_tokens=1 << 27, heads=4),
                                 dict(n_tokens=2 ** 31 - 1, heads=256)])
 def test_batches(lib, kw):
     c = cache(heads=kw.pop("heads", 2))
@@ -54,7 +54,7 @@ def test_batches(lib, kw):
 
 
 @pytest.mark.parametrize("kw", [dict(q_heads=0), dict(q_heads=3), dict(scale=float("nan")), dict(scale=float("inf")), dict(cap=-1.0),
-                                dict(cap=float("nan")), dict(cap=1e-39, scale=3e38), dict(window=-1), dict(q_heads=1 << 30)])
+                                dict(cap=float("nan")), dict(cap=1e-39, scale=3e38), dict(cap=3e38), dict(scale=-3e38), dict(window=-1), dict(q_heads=1 << 30)])
 def test_attention(lib, kw):
     assert calls(lib, cache(), batch(), desc(**kw))[2] in (-1, -2)
     assert lib.otter_hip_kv_attend_workspace_bytes(C.byref(cache()), C.byref(batch()), C.byref(desc(**kw))) == 0
