@@ -693,9 +693,11 @@ size_t otter_hip_linear_workspace_bytes(const otter_hip_linear_t* handle, int x_
 int otter_hip_linear_forward(const otter_hip_linear_t* handle, const float* x, size_t x_stride, int x_rows, const int32_t* index,
                              const int32_t* starts, int rows, float* y, void* workspace, size_t workspace_bytes, void* stream);
 /* For tests and profiling: which launch otter_hip_linear_forward takes for that many rows: 0 the one for few rows, 1 to 3 those for many,
- * 32 x 64, 64 x 64 and 64 x 128 results a wave. The results are the same, bit for bit. */
+ * 32 x 64, 64 x 64 and 64 x 128 results a wave, 4 the one for few rows that quantizes them by itself (the others have a launch for that in
+ * front). The results are the same, bit for bit. */
 int otter_hip_linear_kernel_kind(const otter_hip_linear_t* handle, int rows);
-/* Tuning / test hook: that launch for any number of rows (-1: the choice is automatic). */
+/* Tuning / test hook: that launch for any number of rows (-1: the choice is automatic; 4 where a workgroup's memory holds the codes of 16
+ * rows, else 0). */
 int otter_hip_linear_set_kernel(otter_hip_linear_t* handle, int kind);
 
 #ifdef __cplusplus

@@ -725,7 +725,7 @@ class Linear:
         self._hp = self.h.value  # the handle as the native call path takes it
 
     def kernel_kind(self, rows):
-        """otter_hip_linear_kernel_kind: 0 the launch for few rows, 1 to 3 those for many."""
+        """otter_hip_linear_kernel_kind: 0 and 4 the launches for few rows, 1 to 3 those for many."""
         r = self.L.lib.otter_hip_linear_kernel_kind(self.h, rows)
         self.L._check(min(r, 0))
         return r

@@ -2499,7 +2499,7 @@ int otter_hip_linear_kernel_kind(const otter_hip_linear_t* handle, int rows) {
 }
 
 int otter_hip_linear_set_kernel(otter_hip_linear_t* handle, int kind) {
-    if (!handle || kind < -1 || kind > 3) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_set_kernel: null or no such launch");
+    if (!handle || kind < -1 || kind > 4) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_linear_set_kernel: null or no such launch");
     handle->v.force = kind;
     return OTTER_HIP_OK;
 }

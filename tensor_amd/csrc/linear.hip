@@ -223,6 +223,91 @@ __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
     linear_store<END>(a, row, src < 0 ? 0.f : a.scale[src], n_tile, sum[0], sum[1], o, o_up, linear_quads(a));
 }
 
+// The same launch with the rows' codes found by every workgroup for itself, in LDS, while its first weights are on their way: for the
+// row or two of a decoding step a launch in front of it takes as long as the product (one row of 2048 x 2048: 2.7 and 3.4 us). A row has W / (rows, rounded up to a power of two) waves, or a wave has several rows. 16-byte pieces of a row lie at their index
+// xor (row / 2) % 8, so that the 16 rows of an operand spread over the banks.
+template <int END, int W>
+__global__ void __launch_bounds__(64 * W) linear_rows_kernel(LinearArgs a, const float* __restrict__ x, size_t x_stride) {
+    constexpr int G = END == LINEAR_GATED ? 2 : 1, AHEAD = 4;
+    extern __shared__ __attribute__((aligned(16))) unsigned char lds[];  // codes [row][pieces], then the waves' sums
+    __shared__ float most_of[16][W];
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const unsigned n_tiles = (unsigned)a.w.tiles / G;
+    const int n_tile = (int)(blockIdx.x % n_tiles);
+    const LinearTile t = linear_tile(a, (int)(blockIdx.x / n_tiles), 16);
+    const int count = t.end - t.begin;
+    if (count <= 0) return;
+    const int steps = a.w.steps, in = a.w.in;
+    const int8_t* const w = a.w.w + ((size_t)t.expert * a.w.tiles + (size_t)n_tile * G) * steps * 1024;
+    const unsigned lane16 = (unsigned)lane * 16u;
+    const int each = (steps + W - 1) / W, from = wave * each, to = min(from + each, steps);
+    v4i k[AHEAD][G];
+    const auto load_w = [&](int s) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int h = 0; h < G; ++h) k[u][h] = *reinterpret_cast<const v4i*>(w + ((size_t)h * steps + min(s + u, steps - 1)) * 1024 + lane16);
+    };
+    load_w(min(from, steps - 1));
+    // waves to a row, and the part of the rows' quads that a wave has
+    const int shares = count >= W ? 1 : (count <= 1 ? W : W >> (32 - __clz(count - 1))), share = wave % shares, first = wave / shares, apart = W / shares;
+    const int row_bytes = (int)linear_row_bytes(steps), quads_each = (row_bytes / 4 + shares - 1) / shares;
+    const int q0 = share * quads_each, q1 = min(q0 + quads_each, row_bytes / 4);
+    const bool quads = in % 4 == 0 && x_stride % 4 == 0 && ((size_t)x & 15) == 0;
+    for (int r = first; r < count; r += apart) {
+        const int src = linear_source(a, t.begin + r);
+        const float* const row = x + (size_t)max(src, 0) * x_stride;
+        float most = 0.f;
+        for (int q = q0 + lane; q < q1; q += 64) most = fmaxf(most, most_of_quad(row_quad(row, 4 * q, in, quads)));
+#pragma unroll
+        for (int m = 32; m; m >>= 1) most = fmaxf(most, __shfl_xor(most, m));
+        if (lane == 0) most_of[r][share] = src < 0 ? 0.f : most;
+    }
+    __syncthreads();
+    const auto scale_of_row = [&](int r) {
+        float most = most_of[r][0];
+        for (int n = 1; n < shares; ++n) most = fmaxf(most, most_of[r][n]);
+        return scale_of(most);
+    };
+    for (int r = first; r < count; r += apart) {
+        const int src = linear_source(a, t.begin + r);
+        const float* const row = x + (size_t)max(src, 0) * x_stride;
+        const float s = scale_of_row(r), inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+        for (int q = q0 + lane; q < q1; q += 64) {
+            const int piece = (q >> 2) ^ ((r >> 1) & 7);
+            *reinterpret_cast<int*>(lds + r * row_bytes + piece * 16 + (q & 3) * 4) = codes_of_quad(row_quad(row, 4 * q, in, quads), s, inv);
+        }
+    }
+    __syncthreads();
+    const int mine = min(lane & 15, count - 1);
+    v4i acc[G] = {};
+    for (int s = from; s < to; s += AHEAD) {
+        if (s > from) load_w(s);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (s + u >= to) break;
+            const int piece = ((s + u) * 4 + (lane >> 4)) ^ ((mine >> 1) & 7);
+            const v4i b = *reinterpret_cast<const v4i*>(lds + mine * row_bytes + piece * 16);
+#pragma unroll
+            for (int h = 0; h < G; ++h) acc[h] = __builtin_amdgcn_mfma_i32_16x16x64_i8(k[u][h], b, acc[h], 0, 0, 0);
+        }
+    }
+    __syncthreads();
+    v4i* const sums = reinterpret_cast<v4i*>(lds);
+#pragma unroll
+    for (int h = 0; h < G; ++h) sums[(wave * G + h) * 64 + lane] = acc[h];
+    __syncthreads();
+    const int row = t.begin + (lane & 15);
+    if (wave != 0 || row >= t.end) return;
+    v4i sum[2] = {};
+#pragma unroll
+    for (int h = 0; h < G; ++h)
+#pragma unroll
+        for (int n = 0; n < W; ++n) sum[h] += sums[(n * G + h) * 64 + lane];
+    const LinearOut o = linear_out(a, t.expert, n_tile * G), o_up = linear_out(a, t.expert, n_tile * G + G - 1);
+    linear_store<END>(a, row, scale_of_row(mine), n_tile, sum[0], sum[1], o, o_up, linear_quads(a));
+}
+
 // 64 NT outputs x 16 RT rows a workgroup, 16 NT outputs a wave: the launch for many rows. A wave loads its weights, which no other
 // wave of the workgroup reads, straight into registers, a stage of 128 inputs ahead; the rows' codes, which all four waves read, go
 // through LDS, in lane order too (a 16-byte piece of a row is a lane's). A stage is 8 NT RT matrix instructions a wave against 2 RT KB
@@ -344,13 +429,25 @@ static size_t many_groups(const LinearView& w, const LinearRows& r, int nt, int 
 }
 size_t linear_groups(const LinearView& w, const LinearRows& r) {
     const int k = linear_choice(w, r.rows);
-    return k == 0 ? few_groups(w, r) : k == 1 ? many_groups(w, r, 2, 4) : k == 2 ? many_groups(w, r, 4, 4) : many_groups(w, r, 4, 8);
+    return k == 0 || k == 4 ? few_groups(w, r) : k == 1 ? many_groups(w, r, 2, 4) : k == 2 ? many_groups(w, r, 4, 4) : many_groups(w, r, 4, 8);
 }
 
 template <int W>
 static void launch_few(const LinearArgs& a, const LinearRows& r, hipStream_t stream) {
     const dim3 grid((unsigned)few_groups(a.w, r));
 #define CALL(END) launch(linear_few_kernel<END, W>, grid, dim3(64 * W), 0, stream, a)
+    OHIP_LINEAR_END(CALL)
+#undef CALL
+}
+
+constexpr int ROWS_W = 8;  // waves of linear_rows_kernel
+static int rows_lds(const LinearView& w, int rows) {
+    const int codes = (rows < 16 ? rows : 16) * (int)linear_row_bytes(w.steps), sums = ROWS_W * (w.gated ? 2 : 1) * 1024;
+    return codes > sums ? codes : sums;
+}
+static void launch_rows(const LinearArgs& a, const LinearRows& r, hipStream_t stream) {
+    const dim3 grid((unsigned)few_groups(a.w, r));
+#define CALL(END) launch(linear_rows_kernel<END, ROWS_W>, grid, dim3(64 * ROWS_W), rows_lds(a.w, r.rows), stream, a, r.x, r.x_stride)
     OHIP_LINEAR_END(CALL)
 #undef CALL
 }
@@ -370,7 +467,13 @@ static void launch_many(const LinearArgs& a, const LinearRows& r, hipStream_t st
 // the least traffic, 32 x 64 start the soonest. 4096 x 4096 weights with codes: 128 rows 22 us (few: 26), 512 rows 26.0 (64 x 64: 30.6),
 // 2048 rows 56.2 (32 x 64: 72.6), 8192 rows 193 (64 x 64: 216).
 int linear_choice(const LinearView& w, int rows) {
-    if (w.force >= 0) return w.force;
+    const bool fits = rows_lds(w, rows) <= 65536;
+    if (w.force >= 0) return w.force == 4 && !fits ? 0 : w.force;
+    // Codes within the launch: where a workgroup has few of them to find and the workgroups run beside each other. A row of 2048 x 2048 6.2 ->
+    // 5.1 us, two of 4000 x 4096 8.6 -> 7.8, three 8.6 -> 11.5; a row of 1024 x 16000 6.3 -> 8.4 (one launch behind another without a pause;
+    // called from Python another 2 us less).
+    const int n_tiles = w.tiles / (w.gated ? 2 : 1), most_tiles = rows < 16 * w.experts ? (rows < w.experts ? rows : w.experts) : (rows + 15) / 16;
+    if (fits && (rows <= 2 || (size_t)rows * w.in <= 4096) && (size_t)n_tiles * most_tiles <= 512) return 4;
     const auto row_tiles = [&](int unit) {
         return w.experts == 1 ? (rows + unit - 1) / unit : rows / unit + (rows < w.experts ? rows : w.experts) * 0.5;
     };
@@ -389,13 +492,14 @@ int linear_choice(const LinearView& w, int rows) {
 
 hipError_t run_linear(const LinearView& w, const LinearRows& r, void* workspace, hipStream_t stream) {
     const LinearCodes c = linear_codes(w, r.x_rows, workspace);
-    launch(linear_codes_kernel, dim3((unsigned)r.x_rows), dim3(256), 0, stream, r.x, r.x_stride, w.in, (int)linear_row_bytes(w.steps), c.scale, c.codes);
+    const int choice = linear_choice(w, r.rows);
+    if (choice != 4) launch(linear_codes_kernel, dim3((unsigned)r.x_rows), dim3(256), 0, stream, r.x, r.x_stride, w.in, (int)linear_row_bytes(w.steps), c.scale, c.codes);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
     LinearArgs a{w, c.scale, c.codes, r.index, r.starts, r.x_rows, r.rows, r.y, (size_t)r.rows * w.out * 4 > ((size_t)32 << 20)};
     if (w.act == 1) a.w.act_p0 = __builtin_inff();
     if (w.act == 3) a.w.act_p0 = 6.f;
-    switch (linear_choice(w, r.rows)) {
+    switch (choice) {
     case 0: {
         // eight waves share the inputs where the workgroups alone would leave compute units without work
         const double groups = (double)(w.tiles / (w.gated ? 2 : 1)) * ((r.rows + 15) / 16);
@@ -405,7 +509,8 @@ hipError_t run_linear(const LinearView& w, const LinearRows& r, void* workspace,
     }
     case 1: launch_many<2, 4>(a, r, stream); break;
     case 2: launch_many<4, 4>(a, r, stream); break;
-    default: launch_many<4, 8>(a, r, stream); break;
+    case 3: launch_many<4, 8>(a, r, stream); break;
+    default: launch_rows(a, r, stream); break;
     }
     return hipGetLastError();
 }

@@ -107,6 +107,21 @@ def test_the_largest_sums(hip):
     check(hip, np.random.default_rng(0), x, w, np.full((1, 18), 1e-4, np.float32), None)
 
 
+@pytest.mark.parametrize("rows,k,n,kind", [(1, 2048, 2048, 4), (2, 4000, 1030, 4), (1, 32768, 50, 4), (1, 65600, 50, 0), (4, 1000, 300, 4),
+                                           (5, 1000, 300, 0), (1, 100, 9000, 0), (16, 250, 40, 4)])
+def test_rows_quantized_within_the_launch(hip, rows, k, n, kind):
+    """One to sixteen rows, up to what a workgroup's memory holds; values that are not finite among them."""
+    rng = np.random.default_rng(rows * k)
+    w, s, b = weights(rng, 1, n, k)
+    layer = hip.linear(weight=w, scale=s, bias=b)
+    assert layer.kernel_kind(rows) == kind
+    layer.close()
+    x = rng.normal(0, 1, (rows, k)).astype(np.float32)
+    check(hip, rng, x, w, s, b)
+    x[0, ::7], x[-1, 5], x[-1, k - 1] = 0, np.inf, np.nan
+    check(hip, rng, x, w, s, b)
+
+
 def test_strides(hip):
     rng = np.random.default_rng(7)
     wide = hip.to_device(rng.normal(0, 1, (40, 301)).astype(np.float32))
@@ -130,7 +145,7 @@ def test_a_row_is_the_same_whatever_stands_beside_it(hip):
         assert hip.torch.equal(whole[a:e], layer.forward(x[a:e]))
 
 
-@pytest.mark.parametrize("kind", [0, 1, 2, 3])
+@pytest.mark.parametrize("kind", [0, 1, 2, 3, 4])
 @pytest.mark.parametrize("k,n", [(64, 16), (65, 130), (128, 256), (130, 33), (200, 515), (448, 64), (577, 300), (1000, 270)])
 def test_every_launch(hip, kind, k, n):
     """Each launch at sizes that the choice would not give it: outputs and rows that end inside its tiles, steps of inputs in odd and even
@@ -159,19 +174,19 @@ def test_launches_give_the_same_bits(hip, experts, k, n, rows, gated):
     rng = np.random.default_rng(rows)
     w, s, b = weights(rng, experts, 2 * n if gated else n, k)
     layer = hip.linear(weight=w, scale=s, bias=b, gated=gated)
-    assert layer.kernel_kind(rows) > 0 and layer.kernel_kind(16) == 0
+    assert layer.kernel_kind(rows) in (1, 2, 3)
     cuts = np.sort(rng.integers(0, rows + 1, experts - 1))
     starts = dev(hip, np.concatenate([[3], np.maximum(cuts, 3), [rows]]))
     x = hip.to_device(rng.normal(0, 1, (rows // 2, k)).astype(np.float32))
     index = dev(hip, rng.integers(0, rows // 2, rows))
     want = layer.forward(x, starts, index, out=torch.full((rows, n), 5.0, device=hip.device))
     assert (want[:3] == 5).all() and not (want[3:] == 5).any(1).all()
-    for kind in range(4):
+    for kind in range(5):
         layer.set_kernel(kind)
         assert torch.equal(want, layer.forward(x, starts, index, out=torch.full((rows, n), 5.0, device=hip.device)))
     layer.set_kernel(-1)
     with pytest.raises(capi.HipError):
-        layer.set_kernel(4)
+        layer.set_kernel(5)
     layer.close()
 
 
