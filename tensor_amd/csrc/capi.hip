@@ -2389,7 +2389,7 @@ static int kv_attend_arguments(const char* who, const otter_hip_kv_cache* cache,
     if ((size_t)b->n_tokens * d->q_heads >= (1ull << 31) || tiles * c->heads >= kMostGroups) return fail(OTTER_HIP_ERR_UNSUPPORTED, name + ": batch too large");
     *splits = 1, *bytes = 0;
     if (b->n_seqs == 0 || b->n_tokens == 0) return OTTER_HIP_OK;
-    *splits = kv_attend_splits((int)tiles, c->heads, b->max_pages);
+    *splits = kv_attend_splits((int)tiles, c->heads, c->chunks, b->max_pages);
     if (*splits > 1) {
         const size_t rows = (size_t)b->n_tokens * d->q_heads * *splits;
         *bytes = ((2 * rows + 3) / 4 * 4 + rows * c->dim) * sizeof(float);

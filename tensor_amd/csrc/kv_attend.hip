@@ -334,22 +334,23 @@ constexpr int kv_waves(bool staged) { return !staged || KC > 2 ? 1 : KC == 1 || 
 template <int KC>
 constexpr int kv_staged() { return KC <= 2 ? 2 : 1; }
 template <int KC>
-constexpr int kv_lds_bytes(bool staged) {
-    const int join = 4 * 16 * (64 * KC + 4) * 4 + 4 * 16 * 2 * 4, stage = kv_staged<KC>() * 8 * KC * 1024;
+constexpr int kv_lds_bytes(bool staged, int waves) {
+    const int join = waves * 16 * (64 * KC + 4) * 4 + waves * 16 * 2 * 4, stage = kv_staged<KC>() * 8 * KC * 1024;
     return staged && stage > join ? stage : join;
 }
 
 // 64 rows a workgroup, one key head. Where a sequence has more than 32 rows each wave has a tile of 16 of them; they all read the same
 // pages, which the workgroup stages through LDS, the next ones on their way into registers meanwhile (STAGED; straight from the caches each
-// wave would bring in 16 KB for 48 matrix instructions, and wait for them half of its time). Where it has fewer, two or four waves share a tile's
+// wave would bring in 16 KB for 48 matrix instructions, and wait for them half of its time). Where it has fewer, several waves share a tile's
 // pages out between them, each with its next page's keys and values on their way into registers, and join what they have in LDS.
-template <int KC, int EXTRA, bool STAGED>
-__global__ void __launch_bounds__(256, (kv_waves<KC, EXTRA>(STAGED))) kv_attend_kernel(AttendArgs a) {
-    __shared__ __attribute__((aligned(16))) unsigned char lds[kv_lds_bytes<KC>(STAGED)];
+template <int KC, int EXTRA, bool STAGED, int WAVES>
+__global__ void __launch_bounds__(64 * WAVES, (kv_waves<KC, EXTRA>(STAGED))) kv_attend_kernel(AttendArgs a) {
+    static_assert(!STAGED || WAVES == 4, "the staging is dealt to four waves");
+    __shared__ __attribute__((aligned(16))) unsigned char lds[kv_lds_bytes<KC>(STAGED, WAVES)];
     typedef float JoinedRows[16][64 * KC + 4];
     JoinedRows* const joined = reinterpret_cast<JoinedRows*>(lds);
     typedef float JoinedSums[16][2];
-    JoinedSums* const joined_ml = reinterpret_cast<JoinedSums*>(lds + sizeof(JoinedRows) * 4);
+    JoinedSums* const joined_ml = reinterpret_cast<JoinedSums*>(lds + sizeof(JoinedRows) * WAVES);
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), g = lane >> 4;
     const unsigned lane16 = (unsigned)lane * 16u;
     const int head = (int)(blockIdx.x % (unsigned)a.c.heads);
@@ -358,8 +359,8 @@ __global__ void __launch_bounds__(256, (kv_waves<KC, EXTRA>(STAGED))) kv_attend_
     const int row0 = s.tile * 64, rows = s.count * a.group;
     if (row0 < 0 || row0 >= rows) return;
     const int tiles = (min(rows - row0, 64) + 15) >> 4;      // of 16 rows
-    const int shares = tiles == 1 ? 4 : tiles == 2 ? 2 : 1;  // waves that share a tile's pages
-    const int mine = wave / shares, share = wave % shares;   // (a fourth wave of three tiles has none: it joins the barriers)
+    const int shares = tiles == 1 ? WAVES : tiles == 2 ? WAVES / 2 : WAVES / 4;  // waves that share a tile's pages
+    const int mine = wave / shares, share = wave % shares;                      // (the last of three tiles have none: they join the barriers)
     const bool works = mine < tiles;
     const int r = row0 + mine * 16 + (lane & 15);
     const int row = min(r, rows - 1), token = row / a.group, q_head = head * a.group + row % a.group;
@@ -585,26 +586,33 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const float* __restrict__ 
     if ((int)threadIdx.x < dim) out[(size_t)row * dim + threadIdx.x] = total == 0.f ? 0.f : __fdiv_rn(sum, total);
 }
 
-// Shares that the pages of a tile are cut into, each a workgroup's. A wave reads 16 KB of a page of 128 dims at a time and two
-// workgroups of four fill a compute unit's memory pipe, so there are to be 512 workgroups where the pages give each wave two.
-int kv_attend_splits(int tiles, int heads, int max_pages) {
-    const int have = tiles * heads;
-    const int want = (512 + have - 1) / have, most = max_pages / 8;
-    return want < most ? (want < 1 ? 1 : want) : (most < 1 ? 1 : most);
+// Waves of a workgroup for few rows, and shares that the pages of a tile are cut into, each a workgroup's. Four waves where the tiles give
+// every compute unit two workgroups, as many as their loads need to fill its memory pipe (and over 192 dims, where eight have too few
+// registers); else eight, and as many shares as give every compute unit its eight waves, but four pages to a wave at least: joining the
+// shares takes another launch, as long as four pages do. (One token on 520 tokens, 4 heads of 64: 6.9 us with four waves, 6.2 with eight;
+// on 200 thousand, 4 heads of 128: 44 with four waves and 128 shares, 43 with eight and 64.)
+static int kv_attend_waves(int tiles, int heads, int chunks) { return tiles * heads >= 512 || chunks > 3 ? 4 : 8; }
+int kv_attend_splits(int tiles, int heads, int chunks, int max_pages) {
+    const int have = tiles * heads, waves = kv_attend_waves(tiles, heads, chunks), most = max_pages / (4 * waves);
+    const int want = (2048 / waves + have - 1) / have;
+    return want < most ? want : (most < 1 ? 1 : most);
 }
 int kv_attend_tiles(int n_tokens, int n_seqs, int group) { return (int)((size_t)n_tokens * group / 64) + n_seqs; }
 
-template <int KC, bool STAGED>
+template <int KC, bool STAGED, int WAVES>
 static void launch_attend(const AttendArgs& a, dim3 grid, hipStream_t stream) {
-    if (a.slopes) launch(kv_attend_kernel<KC, 2, STAGED>, grid, dim3(256), 0, stream, a);
-    else if (a.cap != 0.f) launch(kv_attend_kernel<KC, 1, STAGED>, grid, dim3(256), 0, stream, a);
-    else launch(kv_attend_kernel<KC, 0, STAGED>, grid, dim3(256), 0, stream, a);
+    if (a.slopes) launch(kv_attend_kernel<KC, 2, STAGED, WAVES>, grid, dim3(64 * WAVES), 0, stream, a);
+    else if (a.cap != 0.f) launch(kv_attend_kernel<KC, 1, STAGED, WAVES>, grid, dim3(64 * WAVES), 0, stream, a);
+    else launch(kv_attend_kernel<KC, 0, STAGED, WAVES>, grid, dim3(64 * WAVES), 0, stream, a);
 }
 template <int KC>
 static void launch_attend(const AttendArgs& a, dim3 grid, hipStream_t stream) {
     // (staging is for workgroups of more than 32 rows, and LDS for it keeps others out: by the average of the sequences)
-    if ((size_t)a.b.n_tokens * a.group > 32 * (size_t)a.b.n_seqs) launch_attend<KC, true>(a, grid, stream);
-    else launch_attend<KC, false>(a, grid, stream);
+    if ((size_t)a.b.n_tokens * a.group > 32 * (size_t)a.b.n_seqs) launch_attend<KC, true, 4>(a, grid, stream);
+    else if constexpr (KC <= 3) {
+        if (kv_attend_waves(a.tiles, a.c.heads, KC) == 8) launch_attend<KC, false, 8>(a, grid, stream);
+        else launch_attend<KC, false, 4>(a, grid, stream);
+    } else launch_attend<KC, false, 4>(a, grid, stream);
 }
 
 hipError_t run_kv_attend(const KvView& c, const KvBatch& b, const float* q, size_t q_stride, float* out, int q_heads, float scale, float cap,

@@ -107,7 +107,7 @@ hipError_t run_kv_read(const KvView& c, const KvBatch& b, float* k, float* v, hi
 
 // kv_attend.hip
 int kv_attend_tiles(int n_tokens, int n_seqs, int group);
-int kv_attend_splits(int tiles, int heads, int max_pages);
+int kv_attend_splits(int tiles, int heads, int chunks, int max_pages);
 hipError_t run_kv_attend(const KvView& c, const KvBatch& b, const float* q, size_t q_stride, float* out, int q_heads, float scale, float cap,
                          const float* slopes, int causal, int window, int splits, void* workspace, hipStream_t stream);
 

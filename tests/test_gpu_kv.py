@@ -172,8 +172,9 @@ def test_attend_options(hip, kw, dim):
     s.check_attend(s.now, s.normal(s.now, 1, 6)[0], **kw)
 
 
-@pytest.mark.parametrize("dim", [64, 128, 200])
-@pytest.mark.parametrize("lengths", [[(2000, 1)], [(3999, 1), (10, 1), (0, 0), (1000, 1)], [(1500, 9)], [(0, 700), (1300, 1)]])
+@pytest.mark.parametrize("dim", [64, 128, 192, 200])
+@pytest.mark.parametrize("lengths", [[(2000, 1)], [(3999, 1), (10, 1), (0, 0), (1000, 1)], [(1500, 9)], [(0, 700), (1300, 1)], [(9000, 1)],
+                                     [(70, 1), (7000, 2), (0, 1)], [(5000, 40)]])
 def test_attend_of_long_caches(hip, dim, lengths):
     """Few rows: the pages go to several workgroups and are joined behind them, or to the waves of one."""
     s = Setup(hip, np.random.default_rng(11), 1, dim, lengths, front=1, behind=1)
