@@ -8,13 +8,13 @@ namespace ohip {
 
 typedef float v4f __attribute__((ext_vector_type(4)));
 
-// c * was / s rounded half away from zero, exactly: the product of a code and a float is exact in 64 bits, the comparison with the
-// middle between two codes one fused multiply-add.
-__device__ __forceinline__ int code_again(int c, float was, float s) {
-    const double a = __builtin_fabs((double)c * (double)was), d = (double)s;
-    double q = __builtin_floor(a / d + 0.5);
-    if (__builtin_fma(q - 0.5, -d, a) < 0.0) q -= 1.0;
-    else if (__builtin_fma(q + 0.5, -d, a) >= 0.0) q += 1.0;
+// c * was / s rounded half away from zero, exactly: the product of a code and a float is exact in 64 bits, and so is the comparison with the
+// middle between two codes, one fused multiply-add. inv = 1 / s, rounded: what it gives is off by one at most.
+__device__ __forceinline__ int code_again(int c, double was, double s, double inv) {
+    const double a = __builtin_fabs((double)c * was);
+    double q = __builtin_floor(__builtin_fma(a, inv, 0.5));
+    if (__builtin_fma(q - 0.5, -s, a) < 0.0) q -= 1.0;
+    else if (__builtin_fma(q + 0.5, -s, a) >= 0.0) q += 1.0;
     const int i = min((int)q, 127);
     return c < 0 ? -i : i;
 }
@@ -83,8 +83,6 @@ __device__ __forceinline__ void kv_append_block(const KvView& c, const KvTile& t
     typedef KvSquare<KC, VALUES> Square;
     __shared__ float most_of[4];
     const int tid = (int)threadIdx.x;
-    int8_t* const codes = (VALUES ? c.v : c.k) + c.at(t.page, head);
-    float* const scale = (VALUES ? c.vs : c.ks) + (size_t)t.page * c.heads + head;
     const int from = max(t.seq.first - t.position, 0);        // the block's first new token (0: none is older)
     const int to = min(t.seq.length - t.position, KV_BLOCK);  // behind its last
     // row of slot i: begin + (position + i - first)
@@ -97,6 +95,10 @@ __device__ __forceinline__ void kv_append_block(const KvView& c, const KvTile& t
         const Square p(tid + 256 * u);
         load_square(v[u], rows, stride, p.token, p.dim, from, to, c.dim, quads);
     }
+    // (the page's number is on its way with the rows: a call for one token of each sequence is made of such waits)
+    if (t.page < 0) return;
+    int8_t* const codes = (VALUES ? c.v : c.k) + c.at(t.page, head);
+    float* const scale = (VALUES ? c.vs : c.ks) + (size_t)t.page * c.heads + head;
     float was = from > 0 ? *scale : 0.f;
 #pragma unroll
     for (int u = 0; u < KC; ++u)
@@ -111,23 +113,40 @@ __device__ __forceinline__ void kv_append_block(const KvView& c, const KvTile& t
     const float s = fmaxf(was, scale_of(most));
     const bool again = s > was;  // the older tokens' codes change
     const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+    // The older tokens' codes in the new scale, word by word: in a loop, as it is seldom run and would be most of the launch's code.
+    // (A thread's words are those of its squares: what it leaves here it finds below.)
+    if (again && from > 0) {
+        const double inv64 = 1.0 / (double)s;
+#pragma unroll 1
+        for (int n = 0; n < 4 * KC; ++n) {
+            const Square p(tid + 256 * (n >> 2));
+            if (p.token + Square::row(n & 3, 0) >= from) continue;
+            unsigned* const at = reinterpret_cast<unsigned*>(codes + p.at(n & 3));
+            unsigned word = *at;
+#pragma unroll 1
+            for (int e = 0; e < 4; ++e) {  // (the byte in front leaves, its code comes in behind)
+                const int c = byte_of(word, 0);
+                const int code = p.token + Square::row(n & 3, e) >= from ? c : was > 0.f ? code_again(c, was, s, inv64) : 0;
+                word = (word >> 8) | ((unsigned)(code & 0xff) << 24);
+            }
+            *at = word;
+        }
+    }
 #pragma unroll
     for (int u = 0; u < KC; ++u) {
         const Square p(tid + 256 * u);
-        // (a square with neither new tokens nor older ones to change stays as it is, one behind the last too)
-        if (p.token >= to || (p.token + 4 <= from && !again)) continue;
+        if (p.token >= to || p.token + 4 <= from) continue;  // no new token
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             unsigned* const at = reinterpret_cast<unsigned*>(codes + p.at(w));
-            unsigned old = 0, now = 0;
+            unsigned now = 0, old = 0;
             if (p.token < from) old = *at;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const int slot = p.token + Square::row(w, e);
-                int code = 0;
-                if (slot < from) code = !again ? byte_of(old, e) : was > 0.f ? code_again(byte_of(old, e), was, s) : 0;
-                else if (slot < to && s > 0.f) code = code_of(v[u][Square::row(w, e)][Square::column(w, e)], s, inv);
-                now |= (unsigned)(code & 0xff) << (8 * e);
+                const float f = v[u][Square::row(w, e)][Square::column(w, e)];
+                const int code = slot < to && s > 0.f ? code_of(f, s, inv) : 0;
+                now |= (slot < from ? old & (0xffu << (8 * e)) : (unsigned)(code & 0xff) << (8 * e));
             }
             *at = now;
         }
@@ -140,7 +159,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(KvView c, KvBatch b, con
                                                         const float* __restrict__ v, size_t v_stride) {
     const int parts = 2 * c.heads, part = (int)(blockIdx.x % (unsigned)parts);
     const KvTile t = kv_block_of(b, c.n_pages, (int)(blockIdx.x / (unsigned)parts));
-    if (!t.any || t.page < 0) return;
+    if (!t.any) return;
     if (part < c.heads) kv_append_block<KC, false>(c, t, part, k, k_stride);
     else kv_append_block<KC, true>(c, t, part - c.heads, v, v_stride);
 }
