@@ -2376,7 +2376,7 @@ int otter_hip_kv_read(const otter_hip_kv_cache* cache, const otter_hip_kv_batch*
 }
 
 static int kv_attend_arguments(const char* who, const otter_hip_kv_cache* cache, const otter_hip_kv_batch* batch, const otter_hip_kv_attend_desc* d,
-                               KvView* c, KvBatch* b, int* splits, size_t* bytes) {
+                               KvView* c, KvBatch* b, KvPlan* plan, size_t* bytes) {
     const std::string name(who);
     if (int rc = kv_arguments(who, cache, batch, c, b)) return rc;
     if (!d) return fail(OTTER_HIP_ERR_INVALID, name + ": null");
@@ -2387,11 +2387,11 @@ static int kv_attend_arguments(const char* who, const otter_hip_kv_cache* cache,
     if (d->window < 0) return fail(OTTER_HIP_ERR_INVALID, name + ": negative window");
     const size_t group = (size_t)(d->q_heads / c->heads), tiles = (size_t)b->n_tokens * group / 64 + b->n_seqs;
     if ((size_t)b->n_tokens * d->q_heads >= (1ull << 31) || tiles * c->heads >= kMostGroups) return fail(OTTER_HIP_ERR_UNSUPPORTED, name + ": batch too large");
-    *splits = 1, *bytes = 0;
+    *bytes = 0;
     if (b->n_seqs == 0 || b->n_tokens == 0) return OTTER_HIP_OK;
-    *splits = kv_attend_splits((int)tiles, c->heads, c->chunks, b->max_pages);
-    if (*splits > 1) {
-        const size_t rows = (size_t)b->n_tokens * d->q_heads * *splits;
+    *plan = kv_attend_plan(b->n_tokens, b->n_seqs, (int)group, c->heads, c->chunks, d->cap != 0.f || d->slopes, b->max_pages);
+    if (plan->splits > 1) {
+        const size_t rows = (size_t)b->n_tokens * d->q_heads * plan->splits;
         *bytes = ((2 * rows + 3) / 4 * 4 + rows * c->dim) * sizeof(float);
     }
     return OTTER_HIP_OK;
@@ -2400,23 +2400,23 @@ static int kv_attend_arguments(const char* who, const otter_hip_kv_cache* cache,
 size_t otter_hip_kv_attend_workspace_bytes(const otter_hip_kv_cache* cache, const otter_hip_kv_batch* batch, const otter_hip_kv_attend_desc* desc) {
     KvView c;
     KvBatch b;
-    int splits;
+    KvPlan plan;
     size_t bytes = 0;
-    return kv_attend_arguments("otter_hip_kv_attend_workspace_bytes", cache, batch, desc, &c, &b, &splits, &bytes) ? 0 : bytes;
+    return kv_attend_arguments("otter_hip_kv_attend_workspace_bytes", cache, batch, desc, &c, &b, &plan, &bytes) ? 0 : bytes;
 }
 
 int otter_hip_kv_attend(const otter_hip_kv_cache* cache, const otter_hip_kv_batch* batch, const otter_hip_kv_attend_desc* desc, const float* q,
                         size_t q_stride, float* out, void* workspace, size_t workspace_bytes, void* stream) {
     KvView c;
     KvBatch b;
-    int splits;
+    KvPlan plan;
     size_t bytes;
-    if (int rc = kv_attend_arguments("otter_hip_kv_attend", cache, batch, desc, &c, &b, &splits, &bytes)) return rc;
+    if (int rc = kv_attend_arguments("otter_hip_kv_attend", cache, batch, desc, &c, &b, &plan, &bytes)) return rc;
     if (b.n_seqs == 0 || b.n_tokens == 0) return OTTER_HIP_OK;
     if (!q || !out) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_kv_attend: null");
     if (bytes && (!workspace || workspace_bytes < bytes)) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_kv_attend: workspace too small");
     if (bytes && ((size_t)workspace & 15)) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_kv_attend: the workspace must be 16-byte aligned");
-    OHIP_CHECK(run_kv_attend(c, b, q, q_stride, out, desc->q_heads, desc->scale, desc->cap, desc->slopes, desc->causal, desc->window, splits,
+    OHIP_CHECK(run_kv_attend(c, b, q, q_stride, out, desc->q_heads, desc->scale, desc->cap, desc->slopes, desc->causal, desc->window, plan,
                              workspace, (hipStream_t)stream));
     return OTTER_HIP_OK;
 }

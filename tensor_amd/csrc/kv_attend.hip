@@ -326,25 +326,19 @@ __device__ __forceinline__ Pages<NP> pages_at(const KvView& c, int head, PageWal
     return at;
 }
 
-// waves a SIMD that the launch is compiled for: three where that costs no more than a dozen registers spilled (4096 rows on 14 k tokens of
-// 128 dims: 1.33 ms with three, 1.46 with two and two buffers in LDS)
-template <int KC, int EXTRA>
-constexpr int kv_waves(bool staged) { return !staged || KC > 2 ? 1 : KC == 1 || EXTRA == 0 ? 3 : 2; }
-// pages that a workgroup stages at a time: two (see attend_pages) where that leaves LDS for three workgroups a compute unit
-template <int KC>
-constexpr int kv_staged() { return KC <= 2 ? 2 : 1; }
 template <int KC>
 constexpr int kv_lds_bytes(bool staged, int waves) {
-    const int join = waves * 16 * (64 * KC + 4) * 4 + waves * 16 * 2 * 4, stage = kv_staged<KC>() * 8 * KC * 1024;
+    const int join = waves * 16 * (64 * KC + 4) * 4 + waves * 16 * 2 * 4, stage = 2 * 8 * KC * 1024;
     return staged && stage > join ? stage : join;
 }
 
-// 64 rows a workgroup, one key head. Where a sequence has more than 32 rows each wave has a tile of 16 of them; they all read the same
-// pages, which the workgroup stages through LDS, the next ones on their way into registers meanwhile (STAGED; straight from the caches each
-// wave would bring in 16 KB for 48 matrix instructions, and wait for them half of its time). Where it has fewer, several waves share a tile's
-// pages out between them, each with its next page's keys and values on their way into registers, and join what they have in LDS.
+// 64 rows a workgroup, one key head: a wave has a tile of 16 of them, or several waves share a tile's pages out between them and join
+// what they have in LDS. A wave's next page is on its way into registers while it works on one. With STAGED and more than 32 rows the
+// four waves read their pages, which are the same, from LDS, two at a time (see attend_pages), the next two on their way into registers: the
+// faster way only where it leaves room for three workgroups a compute unit and there are as many, by 6 % for 65 to 128 dims (4096 rows on 14
+// thousand tokens: 1.33 ms, 1.45 without, and 1.46 with two buffers in LDS and two workgroups).
 template <int KC, int EXTRA, bool STAGED, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, (kv_waves<KC, EXTRA>(STAGED))) kv_attend_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, STAGED ? 3 : 1) kv_attend_kernel(AttendArgs a) {
     static_assert(!STAGED || WAVES == 4, "the staging is dealt to four waves");
     __shared__ __attribute__((aligned(16))) unsigned char lds[kv_lds_bytes<KC>(STAGED, WAVES)];
     typedef float JoinedRows[16][64 * KC + 4];
@@ -354,10 +348,11 @@ __global__ void __launch_bounds__(64 * WAVES, (kv_waves<KC, EXTRA>(STAGED))) kv_
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6), g = lane >> 4;
     const unsigned lane16 = (unsigned)lane * 16u;
     const int head = (int)(blockIdx.x % (unsigned)a.c.heads);
-    const int tile = a.tiles - 1 - (int)(blockIdx.x / (unsigned)a.c.heads);  // (a causal prompt's last tiles have the most to read)
-    const KvSeq s = kv_locate<true>(a.b.starts, a.b.lengths, a.b.n_seqs, a.b.n_tokens, a.group, 64, 1, tile);
-    const int row0 = s.tile * 64, rows = s.count * a.group;
-    if (row0 < 0 || row0 >= rows) return;
+    const int tile = (int)(blockIdx.x / (unsigned)a.c.heads);
+    const KvSeq s = kv_locate<64, false, true>(a.b.starts, a.b.lengths, a.b.n_seqs, a.b.n_tokens, a.group, tile);
+    const int rows = s.count * a.group, last = ((rows + 63) >> 6) - 1;
+    if (s.tile < 0 || s.tile > last) return;
+    const int row0 = (last - s.tile) * 64;  // (a causal prompt's last rows have the most to read: they come first)
     const int tiles = (min(rows - row0, 64) + 15) >> 4;      // of 16 rows
     const int shares = tiles == 1 ? WAVES : tiles == 2 ? WAVES / 2 : WAVES / 4;  // waves that share a tile's pages
     const int mine = wave / shares, share = wave % shares;                      // (the last of three tiles have none: they join the barriers)
@@ -398,7 +393,7 @@ __global__ void __launch_bounds__(64 * WAVES, (kv_waves<KC, EXTRA>(STAGED))) kv_
     };
     const auto nothing = [] {};
     if (STAGED && shares == 1) {
-        constexpr int NP = kv_staged<KC>(), TILES = NP * 8 * KC, MINE = TILES / 4;
+        constexpr int NP = 2, TILES = NP * 8 * KC, MINE = TILES / 4;
         v4i* const buffer = reinterpret_cast<v4i*>(lds);  // [page][4 KC tiles of keys, as many of values][lane]
         const int p0 = s.first + row0 / a.group, p1 = s.first + (min(row0 + 64, rows) - 1) / a.group;
         deal(sees_from(p0), sees_to(p1), (int)blockIdx.y, a.splits);
@@ -412,8 +407,7 @@ __global__ void __launch_bounds__(64 * WAVES, (kv_waves<KC, EXTRA>(STAGED))) kv_
 #pragma unroll
                 for (int u = 0; u < MINE; ++u) {
                     const int j = wave * MINE + u, n = j / (8 * KC), of = j % (8 * KC);
-                    const int8_t* const k = NP == 2 && n ? kp[NP - 1] : kp[0];
-                    const int8_t* const v = NP == 2 && n ? vp[NP - 1] : vp[0];
+                    const int8_t *const k = n ? kp[1] : kp[0], *const v = n ? vp[1] : vp[0];
                     mine_of[u] = *reinterpret_cast<const v4i*>((of < 4 * KC ? k + of * 1024 : v + (of - 4 * KC) * 1024) + lane16);
                 }
             };
@@ -526,17 +520,19 @@ __global__ void __launch_bounds__(64 * WAVES, (kv_waves<KC, EXTRA>(STAGED))) kv_
     }
 }
 
-// The splits of a row joined: a workgroup for each (token, query head), a quarter of the splits for each of its waves, whose sums meet
-// in LDS. A wave walks its splits a few at a time, so that their loads are in flight together: one by one, by a single wave, 128 splits
-// of 28 rows took 110 us, three times the attention itself.
+// The splits of a row joined, a row being a (token, query head): by a wave, or where they are many by the four of a workgroup, a quarter
+// of the splits each, whose sums meet in LDS. A wave walks its splits eight at a time, so that their loads are in flight together. (One by
+// one, by a single wave, 128 splits of 28 rows took 110 us; a workgroup for each of 12800 rows of two splits 25 us.)
+template <int WAVES>
 __global__ void __launch_bounds__(256) kv_join_kernel(const float* __restrict__ part_o, const float* __restrict__ part_ml, float* __restrict__ out,
                                                       const int32_t* __restrict__ starts, int n_seqs, int n_rows, int q_heads, int dim, int splits) {
     __shared__ float sums[4][256];
     __shared__ float share_of[4][2];
-    const int row = (int)blockIdx.x, lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
+    const int row = WAVES == 4 ? (int)blockIdx.x : (int)blockIdx.x * 4 + wave, share = WAVES == 4 ? wave : 0;
     const int token = row / q_heads;
-    if (token < starts[0] || token >= starts[n_seqs]) return;  // rows of no sequence stay as they were
-    const int each = (splits + 3) / 4, from = min(wave * each, splits), to = min(from + each, splits);
+    if (row >= n_rows || token < starts[0] || token >= starts[n_seqs]) return;  // rows of no sequence stay as they were
+    const int each = (splits + WAVES - 1) / WAVES, from = min(share * each, splits), to = min(from + each, splits);
     // the wave's largest maximum; NaN weights have none: -infinity and a sum that is not 0
     float m = -__builtin_inff();
     for (int n = from + lane; n < to; n += 64) m = fmaxf(m, part_ml[2 * ((size_t)n * n_rows + row)]);
@@ -560,7 +556,7 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const float* __restrict__ 
                 k[i] = n + i < count ? __shfl(keep, n + i) : 0.f;  // (of an empty split 0 too: its sums are not written)
                 const float* const at = part_o + ((size_t)(n0 + min(n + i, count - 1)) * n_rows + row) * dim;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) f[i][e] = lane + 64 * e < dim ? at[lane + 64 * e] : 0.f;
+                for (int e = 0; e < 4; ++e) f[i][e] = n + i < count && lane + 64 * e < dim ? at[lane + 64 * e] : 0.f;
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -570,53 +566,69 @@ __global__ void __launch_bounds__(256) kv_join_kernel(const float* __restrict__ 
     }
 #pragma unroll
     for (int k = 32; k; k >>= 1) l = __fadd_rn(l, __shfl_xor(l, k));
+    if constexpr (WAVES == 1) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sums[wave][lane + 64 * e] = o[e];
-    if (lane == 0) share_of[wave][0] = m, share_of[wave][1] = l;
-    __syncthreads();
-    m = fmaxf(fmaxf(share_of[0][0], share_of[1][0]), fmaxf(share_of[2][0], share_of[3][0]));
-    float total = 0.f, sum = 0.f;
+        for (int e = 0; e < 4; ++e)
+            if (lane + 64 * e < dim) out[(size_t)row * dim + lane + 64 * e] = l == 0.f ? 0.f : __fdiv_rn(o[e], l);
+    } else {
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        const float lw = share_of[w][1], mw = share_of[w][0];
-        const float keep = lw == 0.f ? 0.f : mw == -__builtin_inff() ? 1.f : fast_exp2(__fadd_rn(mw, -m));
-        total = __fmaf_rn(lw, keep, total);
-        sum = __fmaf_rn(sums[w][threadIdx.x], keep, sum);
+        for (int e = 0; e < 4; ++e) sums[wave][lane + 64 * e] = o[e];
+        if (lane == 0) share_of[wave][0] = m, share_of[wave][1] = l;
+        __syncthreads();
+        m = fmaxf(fmaxf(share_of[0][0], share_of[1][0]), fmaxf(share_of[2][0], share_of[3][0]));
+        float total = 0.f, sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float lw = share_of[w][1], mw = share_of[w][0];
+            const float keep = lw == 0.f ? 0.f : mw == -__builtin_inff() ? 1.f : fast_exp2(__fadd_rn(mw, -m));
+            total = __fmaf_rn(lw, keep, total);
+            sum = __fmaf_rn(sums[w][threadIdx.x], keep, sum);
+        }
+        if ((int)threadIdx.x < dim) out[(size_t)row * dim + threadIdx.x] = total == 0.f ? 0.f : __fdiv_rn(sum, total);
     }
-    if ((int)threadIdx.x < dim) out[(size_t)row * dim + threadIdx.x] = total == 0.f ? 0.f : __fdiv_rn(sum, total);
 }
 
-// Waves of a workgroup for few rows, and shares that the pages of a tile are cut into, each a workgroup's. Four waves where the tiles give
-// every compute unit two workgroups, as many as their loads need to fill its memory pipe (and over 192 dims, where eight have too few
-// registers); else eight, and as many shares as give every compute unit its eight waves, but four pages to a wave at least: joining the
-// shares takes another launch, as long as four pages do. (One token on 520 tokens, 4 heads of 64: 6.9 us with four waves, 6.2 with eight;
-// on 200 thousand, 4 heads of 128: 44 with four waves and 128 shares, 43 with eight and 64.)
-static int kv_attend_waves(int tiles, int heads, int chunks) { return tiles * heads >= 512 || chunks > 3 ? 4 : 8; }
-int kv_attend_splits(int tiles, int heads, int chunks, int max_pages) {
-    const int have = tiles * heads, waves = kv_attend_waves(tiles, heads, chunks), most = max_pages / (4 * waves);
-    const int want = (2048 / waves + have - 1) / have;
-    return want < most ? want : (most < 1 ? 1 : most);
+// How a batch is launched, by the tiles that its rows fill if they are spread evenly: the sizes of its sequences are on the GPU.
+//   staged  from three workgroups a compute unit on, more being there to follow (extra: cap or slopes, which take its registers)
+//   waves   of a workgroup: four where the tiles give every compute unit more than one, as many as their loads need to fill its memory pipe
+//           (and over 192 dims, where eight have too few registers), else eight. One token on 520 tokens, 4 heads of 64: 6.9 us with
+//           four, 6.2 with eight; 16 x 64 rows on 4000 tokens, 8 heads of 128: 86 and 70
+//   splits  shares that the pages of a tile are cut into, each a workgroup's: as many as give the compute units eight waves at the most, but
+//           four pages to a wave at least: joining the shares takes another launch, as long as four pages do. 64 rows on 16 thousand tokens:
+//           240 us in one share, 53 in eight
+KvPlan kv_attend_plan(int n_tokens, int n_seqs, int group, int heads, int chunks, bool extra, int max_pages) {
+    const size_t rows = (size_t)n_tokens * group, even = (rows + 63) / 64, seqs = (size_t)n_seqs;
+    const size_t have = (even > seqs ? even : seqs) * heads;
+    KvPlan p;
+    p.staged = chunks == 2 && !extra && have >= 1024 && rows > 32 * seqs;
+    p.waves = have > 256 || chunks > 3 ? 4 : 8;
+    const int tiles = rows <= 16 * seqs ? 1 : rows <= 32 * seqs ? 2 : 4;  // of 16 rows, which the waves of a workgroup are dealt to
+    const size_t fill = 2048 / p.waves / have, want = have > 256 || fill < 1 ? 1 : fill, most = (size_t)max_pages / (4 * (p.waves / tiles));
+    p.splits = (int)(want < most ? want : most < 1 ? 1 : most);
+    return p;
 }
 int kv_attend_tiles(int n_tokens, int n_seqs, int group) { return (int)((size_t)n_tokens * group / 64) + n_seqs; }
 
-template <int KC, bool STAGED, int WAVES>
+template <int KC, int WAVES>
 static void launch_attend(const AttendArgs& a, dim3 grid, hipStream_t stream) {
-    if (a.slopes) launch(kv_attend_kernel<KC, 2, STAGED, WAVES>, grid, dim3(64 * WAVES), 0, stream, a);
-    else if (a.cap != 0.f) launch(kv_attend_kernel<KC, 1, STAGED, WAVES>, grid, dim3(64 * WAVES), 0, stream, a);
-    else launch(kv_attend_kernel<KC, 0, STAGED, WAVES>, grid, dim3(64 * WAVES), 0, stream, a);
+    if (a.slopes) launch(kv_attend_kernel<KC, 2, false, WAVES>, grid, dim3(64 * WAVES), 0, stream, a);
+    else if (a.cap != 0.f) launch(kv_attend_kernel<KC, 1, false, WAVES>, grid, dim3(64 * WAVES), 0, stream, a);
+    else launch(kv_attend_kernel<KC, 0, false, WAVES>, grid, dim3(64 * WAVES), 0, stream, a);
 }
 template <int KC>
-static void launch_attend(const AttendArgs& a, dim3 grid, hipStream_t stream) {
-    // (staging is for workgroups of more than 32 rows, and LDS for it keeps others out: by the average of the sequences)
-    if ((size_t)a.b.n_tokens * a.group > 32 * (size_t)a.b.n_seqs) launch_attend<KC, true, 4>(a, grid, stream);
-    else if constexpr (KC <= 3) {
-        if (kv_attend_waves(a.tiles, a.c.heads, KC) == 8) launch_attend<KC, false, 8>(a, grid, stream);
-        else launch_attend<KC, false, 4>(a, grid, stream);
-    } else launch_attend<KC, false, 4>(a, grid, stream);
+static void launch_attend(const AttendArgs& a, const KvPlan& p, dim3 grid, hipStream_t stream) {
+    if constexpr (KC == 2) {
+        if (p.staged) return launch(kv_attend_kernel<2, 0, true, 4>, grid, dim3(256), 0, stream, a);
+    }
+    if constexpr (KC <= 3) {
+        if (p.waves == 8) return launch_attend<KC, 8>(a, grid, stream);
+    }
+    launch_attend<KC, 4>(a, grid, stream);
 }
 
 hipError_t run_kv_attend(const KvView& c, const KvBatch& b, const float* q, size_t q_stride, float* out, int q_heads, float scale, float cap,
-                         const float* slopes, int causal, int window, int splits, void* workspace, hipStream_t stream) {
+                         const float* slopes, int causal, int window, const KvPlan& plan, void* workspace, hipStream_t stream) {
+    const int splits = plan.splits;
     AttendArgs a;
     a.c = c, a.b = b, a.q = q, a.q_stride = q_stride, a.out = out, a.q_heads = q_heads, a.group = q_heads / c.heads;
     a.scale = cap != 0.f ? scale / cap : scale * LOG2E;
@@ -628,15 +640,19 @@ hipError_t run_kv_attend(const KvView& c, const KvBatch& b, const float* q, size
     a.part_o = a.part_ml + (splits > 1 ? (2 * rows * splits + 3) / 4 * 4 : 0);
     const dim3 grid((unsigned)a.tiles * (unsigned)c.heads, (unsigned)splits);
     switch (c.chunks) {
-    case 1: launch_attend<1>(a, grid, stream); break;
-    case 2: launch_attend<2>(a, grid, stream); break;
-    case 3: launch_attend<3>(a, grid, stream); break;
-    default: launch_attend<4>(a, grid, stream); break;
+    case 1: launch_attend<1>(a, plan, grid, stream); break;
+    case 2: launch_attend<2>(a, plan, grid, stream); break;
+    case 3: launch_attend<3>(a, plan, grid, stream); break;
+    default: launch_attend<4>(a, plan, grid, stream); break;
     }
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || splits == 1) return e;
-    launch(kv_join_kernel, dim3((unsigned)rows), dim3(256), 0, stream, (const float*)a.part_o, (const float*)a.part_ml, out, b.starts,
-           b.n_seqs, (int)rows, q_heads, c.dim, splits);
+    const auto join = [&](auto kernel, size_t groups) {
+        launch(kernel, dim3((unsigned)groups), dim3(256), 0, stream, (const float*)a.part_o, (const float*)a.part_ml, out, b.starts, b.n_seqs, (int)rows,
+               q_heads, c.dim, splits);
+    };
+    if (splits > 16) join(kv_join_kernel<4>, rows);
+    else join(kv_join_kernel<1>, (rows + 3) / 4);
     return hipGetLastError();
 }
 

@@ -30,7 +30,7 @@ struct KvTile {
 // tile -> (sequence, block)
 __device__ __forceinline__ KvTile kv_block_of(const KvBatch& b, int n_pages, int tile) {
     KvTile t;
-    t.seq = kv_locate<true>(b.starts, b.lengths, b.n_seqs, b.n_tokens, 1, KV_BLOCK, 2, tile);
+    t.seq = kv_locate<KV_BLOCK, true, true>(b.starts, b.lengths, b.n_seqs, b.n_tokens, 1, tile);
     const int block = (t.seq.first >> 6) + t.seq.tile;
     t.any = t.seq.tile >= 0 && t.seq.count > 0 && block <= ((t.seq.length - 1) >> 6);
     t.position = block * KV_BLOCK;

@@ -46,30 +46,54 @@ struct KvSeq {
     int tile;          // of the sequence (below 0: of none)
 };
 
-// Work is dealt to tiles of `unit` rows of a sequence without a list of them: sequence i's tiles begin at starts[i] * mul / unit +
-// slack * i, which leaves each at least as many as it needs (ceil(n / unit) <= floor difference + 1, and one more where a tile is
-// aligned to positions, not to rows). The largest i whose tiles begin at or before `tile`, by the lanes of a wave: a load for each
-// 64-fold of sequences, and what is to be known of the one that is found comes with the last of them.
-__device__ __forceinline__ int kv_tile_base(int start, int i, int limit, int mul, int unit, int slack) {
-    return (int)((unsigned)(min(max(start, 0), limit) * mul) / (unsigned)unit) + slack * i;
+// The sum over this lane and those below it.
+__device__ __forceinline__ int lanes_below(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, true);   // a row of 16 lanes: one to the right,
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, true);   // two,
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, true);   // four,
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, true);   // eight
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // the last of rows 0 and 2 into rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // the last of row 1 into rows 2 and 3
+    return v;
 }
-template <bool LENGTHS>
-__device__ __forceinline__ KvSeq kv_locate(const int32_t* starts, const int32_t* lengths, int n, int limit, int mul, int unit, int slack, int tile) {
+
+// Work is dealt to tiles of UNIT rows of a sequence (mul rows for each of `starts`; BLOCKS: to the blocks of 64 positions that its rows lie
+// in) without a list of them, by the lanes of a wave, and what is to be known of the sequence that is found comes along.
+// Up to 64 sequences: a lane counts the tiles of one, and a sum over the lanes says whose the tile is. More: sequence i's tiles
+// begin at starts[i] * mul / UNIT + SLACK * i, which leaves each at least as many as it needs (ceil(n / UNIT) <= floor difference + 1, and
+// one more where blocks are aligned to positions), and a load for each 64-fold of sequences finds the largest i whose tiles begin at or
+// before the tile. The first way leaves no tiles empty but the grid's last ones: workgroups are handed to the shader engines in
+// turn, and empty ones among them left some engines with one more than others (32 sequences of 5 query heads to a key head, 8 key heads,
+// one workgroup a compute unit: 65 us, with 4 query heads 47).
+template <int UNIT, bool BLOCKS, bool LENGTHS>
+__device__ __forceinline__ KvSeq kv_locate(const int32_t* starts, const int32_t* lengths, int n, int limit, int mul, int tile) {
+    constexpr int SLACK = BLOCKS ? 2 : 1;
     const int lane = (int)(threadIdx.x & 63);
     int lo = 0;
+    const bool few = n <= 64;
     for (;;) {
         const int step = (n + 63) >> 6, i = lane * step, at = lo + min(i, n - 1);
-        const int from = starts[at], to = starts[at + 1];
+        const int from = min(max(starts[at], 0), limit), count = min(max(starts[at + 1], from), limit) - from;
         int length = 0;
-        if constexpr (LENGTHS) length = lengths[at];
-        const int base = kv_tile_base(from, at, limit, mul, unit, slack);
-        const int k = max(__popcll(__ballot(i < n && base <= tile)), 1) - 1;
+        if constexpr (LENGTHS) length = max(lengths[at], 0);
+        int base, k;
+        if (few) {
+            int tiles = BLOCKS ? ((length - 1) >> 6) - ((length - count) >> 6) + 1 : (int)((unsigned)(count * mul + UNIT - 1) / UNIT);
+            if (i >= n || count == 0) tiles = 0;
+            base = lanes_below(tiles) - tiles;
+            const unsigned long long mine = __ballot(tiles > 0 && base <= tile);
+            k = mine ? 63 - __builtin_clzll(mine) : 0;
+            if (!mine) base = tile + 1;  // (no sequence has rows)
+        } else {
+            base = (int)((unsigned)(from * mul) / (unsigned)UNIT) + SLACK * at;
+            k = max(__popcll(__ballot(i < n && base <= tile)), 1) - 1;
+        }
         if (step == 1) {
             KvSeq s;
             s.index = __builtin_amdgcn_readfirstlane(lo + k);
-            s.begin = min(max(__builtin_amdgcn_readlane(from, k), 0), limit);
-            s.count = min(max(__builtin_amdgcn_readlane(to, k), s.begin), limit) - s.begin;
-            s.length = max(__builtin_amdgcn_readlane(length, k), 0);
+            s.begin = __builtin_amdgcn_readlane(from, k);
+            s.count = __builtin_amdgcn_readlane(count, k);
+            s.length = __builtin_amdgcn_readlane(length, k);
             s.first = s.length - s.count;
             s.tile = tile - __builtin_amdgcn_readlane(base, k);
             return s;
@@ -107,8 +131,12 @@ hipError_t run_kv_read(const KvView& c, const KvBatch& b, float* k, float* v, hi
 
 // kv_attend.hip
 int kv_attend_tiles(int n_tokens, int n_seqs, int group);
-int kv_attend_splits(int tiles, int heads, int chunks, int max_pages);
+struct KvPlan {
+    bool staged;
+    int waves, splits;
+};
+KvPlan kv_attend_plan(int n_tokens, int n_seqs, int group, int heads, int chunks, bool extra, int max_pages);
 hipError_t run_kv_attend(const KvView& c, const KvBatch& b, const float* q, size_t q_stride, float* out, int q_heads, float scale, float cap,
-                         const float* slopes, int causal, int window, int splits, void* workspace, hipStream_t stream);
+                         const float* slopes, int causal, int window, const KvPlan& plan, void* workspace, hipStream_t stream);
 
 }  // namespace ohip

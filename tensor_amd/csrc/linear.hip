@@ -84,21 +84,22 @@ struct LinearArgs {
     bool streams;
 };
 
-// Expert and rows of a tile of `unit` rows: [begin, end), empty where the tile is behind its expert's rows.
+// Expert and rows of a tile of UNIT rows: [begin, end), empty where the tile is behind its expert's rows.
 struct LinearTile {
     int expert, begin, end;
 };
-__device__ __forceinline__ LinearTile linear_tile(const LinearArgs& a, int tile, int unit) {
+template <int UNIT>
+__device__ __forceinline__ LinearTile linear_tile(const LinearArgs& a, int tile) {
     LinearTile t;
     if (!a.starts) {
-        t.expert = 0, t.begin = tile * unit, t.end = min(t.begin + unit, a.rows);
+        t.expert = 0, t.begin = tile * UNIT, t.end = min(t.begin + UNIT, a.rows);
         return t;
     }
-    const KvSeq s = kv_locate<false>(a.starts, nullptr, a.w.experts, a.rows, 1, unit, 1, tile);
+    const KvSeq s = kv_locate<UNIT, false, false>(a.starts, nullptr, a.w.experts, a.rows, 1, tile);
     t.expert = s.index;
     const int to = s.begin + s.count;
-    t.begin = s.tile < 0 ? to : min(s.begin + s.tile * unit, to);
-    t.end = min(t.begin + unit, to);
+    t.begin = s.tile < 0 ? to : min(s.begin + s.tile * UNIT, to);
+    t.end = min(t.begin + UNIT, to);
     return t;
 }
 static int linear_row_tiles(const LinearView& w, const LinearRows& r, int unit) {
@@ -185,7 +186,7 @@ __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const unsigned n_tiles = (unsigned)a.w.tiles / G;
     const int n_tile = (int)(blockIdx.x % n_tiles);
-    const LinearTile t = linear_tile(a, (int)(blockIdx.x / n_tiles), 16);
+    const LinearTile t = linear_tile<16>(a, (int)(blockIdx.x / n_tiles));
     if (t.begin >= t.end) return;
     const int steps = a.w.steps;
     const int8_t* const w = a.w.w + ((size_t)t.expert * a.w.tiles + (size_t)n_tile * G) * steps * 1024;
@@ -234,7 +235,7 @@ __global__ void __launch_bounds__(64 * W) linear_rows_kernel(LinearArgs a, const
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const unsigned n_tiles = (unsigned)a.w.tiles / G;
     const int n_tile = (int)(blockIdx.x % n_tiles);
-    const LinearTile t = linear_tile(a, (int)(blockIdx.x / n_tiles), 16);
+    const LinearTile t = linear_tile<16>(a, (int)(blockIdx.x / n_tiles));
     const int count = t.end - t.begin;
     if (count <= 0) return;
     const int steps = a.w.steps, in = a.w.in;
@@ -318,7 +319,7 @@ __global__ void __launch_bounds__(256, 2) linear_many_kernel(LinearArgs a) {
     __shared__ v4i rows[3][RT][2][64];
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
     const unsigned n_blocks = (unsigned)(a.w.tiles + 4 * NT - 1) / (4 * NT);
-    const LinearTile t = linear_tile(a, (int)(blockIdx.x / n_blocks), 16 * RT);
+    const LinearTile t = linear_tile<16 * RT>(a, (int)(blockIdx.x / n_blocks));
     if (t.begin >= t.end) return;
     const int tile0 = ((int)(blockIdx.x % n_blocks) * 4 + wave) * NT, steps = a.w.steps;
     const size_t row_bytes = linear_row_bytes(steps);
