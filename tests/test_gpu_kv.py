@@ -183,6 +183,48 @@ def test_attend_of_long_caches(hip, dim, lengths):
         s.check_attend(s.now, s.normal(s.now, 1, 3)[0], **kw)
 
 
+@pytest.mark.parametrize("dim,kw", [(128, dict()), (80, dict()), (128, dict(window=300)), (100, dict(causal=False)), (128, dict(cap=5.0)),
+                                    (128, dict(slopes=True, cap=30.0)), (64, dict()), (64, dict(slopes=True)), (192, dict()), (256, dict(window=500))])
+def test_attend_of_many_rows(hip, dim, kw):
+    """Batches that fill the GPU several times, ragged, from one row to 1500 a sequence; a sample of rows, the first and the last of each
+    sequence and of some tiles among them, against the model."""
+    rng = np.random.default_rng(dim)
+    heads = 16
+    lengths = [(0, 1500), (300, 1333), (100, 1), (0, 17), (70, 1111), (0, 0), (500, 48), (0, 300)]
+    s = Setup(hip, rng, heads, dim, lengths, front=1, behind=2)
+    s.append(s.now, *s.normal(s.now, 2))
+    q = s.normal(s.now, 1, heads)[0]
+    if kw.get("slopes"):
+        kw = dict(kw, slopes=rng.uniform(0.01, 0.5, heads).astype(np.float32))
+    starts = s.now[0]
+    rows = {int(r) for a, b in zip(starts, starts[1:]) if b > a for r in (a, b - 1, a + (b - a) // 64 * 64, max(a, b - 17))} | \
+        set(map(int, rng.integers(starts[0], starts[-1], 40)))
+    rows = [r for r in rows if starts[0] <= r < starts[-1]]
+    only = {(r, int(h)) for r in rows for h in rng.integers(0, heads, 2)}
+    into = rng.normal(0, 1, q.shape).astype(np.float32)
+    dkw = dict(kw, slopes=None if kw.get("slopes") is None else hip.to_device(kw["slopes"]))
+    got = s.cache.attend(s.now[3], hip.to_device(q), out=hip.to_device(into), **dkw).cpu().numpy()
+    np.testing.assert_array_equal(got[:1], into[:1])
+    np.testing.assert_array_equal(got[-2:], into[-2:])
+    want, bound = s.model.attend(starts, s.now[1], s.table, q, into, only=only, **kw)
+    r, h = (np.array(t) for t in zip(*sorted(only)))
+    check_close(got[r, h], want[r, h], bound[r, h])
+
+
+@pytest.mark.parametrize("seqs", [64, 65, 150, 4500])
+def test_many_sequences(hip, seqs):
+    """Up to 64 sequences and beyond, several 64-folds of them; some without rows, some without tokens."""
+    rng = np.random.default_rng(seqs)
+    most = 140 if seqs < 1000 else 2
+    lengths = [(int(rng.integers(0, most)), int(rng.integers(0, most) * rng.integers(0, 2))) for _ in range(seqs)]
+    s = Setup(hip, rng, 1, 32, lengths, front=1, behind=1)
+    s.append(s.now, *s.normal(s.now, 2))
+    s.check_read(s.now)
+    s.check_attend(s.now, s.normal(s.now, 1, 1)[0])
+    if seqs < 1000:
+        s.check_attend(s.now, s.normal(s.now, 1, 3)[0], window=40)
+
+
 @pytest.mark.parametrize("dim", [64, 128, 192, 256])
 @pytest.mark.parametrize("lengths", [[(70 * i, 1) for i in range(20)] + [(300, 90)], [(0, 400), (1000, 30)], [(500, 33), (5, 17), (0, 300)]])
 def test_attend_of_few_and_many_rows_together(hip, dim, lengths):

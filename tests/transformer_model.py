@@ -80,8 +80,8 @@ class Cache:
             k[starts[i]:starts[i + 1]], v[starts[i]:starts[i + 1]], _ = self.tokens(i, table, np.arange(lengths[i] - n, lengths[i]))
         return k, v
 
-    def attend(self, starts, lengths, table, q, into, *, scale=None, cap=0.0, causal=True, window=0, slopes=None):
-        """The result and a bound on how far the launch may be off, see the comment at the bound."""
+    def attend(self, starts, lengths, table, q, into, *, scale=None, cap=0.0, causal=True, window=0, slopes=None, only=None):
+        """The result and a bound on how far the launch may be off, see the comment at the bound. only: the (row, head) to work out."""
         out, bound = into.astype(np.float64), np.zeros(into.shape)
         heads = q.shape[1]
         group = heads // self.heads
@@ -91,10 +91,14 @@ class Cache:
             k, v, there = self.tokens(i, table, np.arange(total))
             j = np.arange(total)
             for r in range(n):
+                if only is not None and not any((int(starts[i]) + r, h) in only for h in range(heads)):
+                    continue
                 p = total - n + r
                 sees = there & ((j <= p) if causal else True) & ((p - j < window) if window else True) & (p >= 0)
                 for h in range(heads):
                     row = starts[i] + r
+                    if only is not None and (int(row), h) not in only:
+                        continue
                     out[row, h] = 0
                     x = q[row, h].astype(np.float64)
                     if not sees.any():
