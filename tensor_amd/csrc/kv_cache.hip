@@ -59,7 +59,7 @@ struct KvSquare {
 };
 
 // [rows][dims] of a square; rows outside [from, to) and dims behind the last are 0. `quads`: rows at multiples of 16 bytes, whole quads.
-__device__ __forceinline__ void load_square(float (&v)[4][4], const float* __restrict__ rows, size_t stride, int token, int dim, int from, int to, int dims,
+__device__ __forceinline__ void load_square(float (&v)[16], const float* __restrict__ rows, size_t stride, int token, int dim, int from, int to, int dims,
                                             bool quads) {
 #pragma unroll
     for (int r = 0; r < 4; ++r) {
@@ -74,7 +74,7 @@ __device__ __forceinline__ void load_square(float (&v)[4][4], const float* __res
             if (dim + 2 < dims) f.z = p[2];
             if (dim + 3 < dims) f.w = p[3];
         }
-        v[r][0] = f.x, v[r][1] = f.y, v[r][2] = f.z, v[r][3] = f.w;
+        v[4 * r] = f.x, v[4 * r + 1] = f.y, v[4 * r + 2] = f.z, v[4 * r + 3] = f.w;
     }
 }
 
@@ -88,7 +88,7 @@ __device__ __forceinline__ void kv_append_block(const KvView& c, const KvTile& t
     // row of slot i: begin + (position + i - first)
     const float* const rows = x + ((ptrdiff_t)t.seq.begin + t.position - t.seq.first) * (ptrdiff_t)stride + (size_t)head * c.dim;
     const bool quads = c.dim % 4 == 0 && stride % 4 == 0 && ((size_t)x & 15) == 0;
-    float v[KC][4][4];
+    float v[KC][16];
     float most = 0.f;
 #pragma unroll
     for (int u = 0; u < KC; ++u) {
@@ -101,9 +101,7 @@ __device__ __forceinline__ void kv_append_block(const KvView& c, const KvTile& t
     float* const scale = (VALUES ? c.vs : c.ks) + (size_t)t.page * c.heads + head;
     float was = from > 0 ? *scale : 0.f;
 #pragma unroll
-    for (int u = 0; u < KC; ++u)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) most = fmaxf(most, finite_size(v[u][e >> 2][e & 3]));
+    for (int u = 0; u < KC; ++u) most = fmaxf(most, largest_size(v[u]));
 #pragma unroll
     for (int m = 32; m; m >>= 1) most = fmaxf(most, __shfl_xor(most, m));
     if ((tid & 63) == 0) most_of[tid >> 6] = most;
@@ -112,7 +110,7 @@ __device__ __forceinline__ void kv_append_block(const KvView& c, const KvTile& t
     if (!(was >= KV_LEAST_SCALE && was < __builtin_inff())) was = 0.f;
     const float s = fmaxf(was, scale_of(most));
     const bool again = s > was;  // the older tokens' codes change
-    const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+    const Coder coder(s);
     // The older tokens' codes in the new scale, word by word: in a loop, as it is seldom run and would be most of the launch's code.
     // (A thread's words are those of its squares: what it leaves here it finds below.)
     if (again && from > 0) {
@@ -132,23 +130,47 @@ __device__ __forceinline__ void kv_append_block(const KvView& c, const KvTile& t
             *at = word;
         }
     }
+    // (tokens in front of a word's first new one keep their bytes)
+    const auto older = [&](const Square& p, int w) {
+        unsigned mask = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) mask |= p.token + Square::row(w, e) < from ? 0xffu << (8 * e) : 0u;
+        return mask;
+    };
+    bool doubtful = false;
 #pragma unroll
     for (int u = 0; u < KC; ++u) {
         const Square p(tid + 256 * u);
         if (p.token >= to || p.token + 4 <= from) continue;  // no new token
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            unsigned* const at = reinterpret_cast<unsigned*>(codes + p.at(w));
-            unsigned now = 0, old = 0;
-            if (p.token < from) old = *at;
+            float f[4];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int slot = p.token + Square::row(w, e);
-                const float f = v[u][Square::row(w, e)][Square::column(w, e)];
-                const int code = slot < to && s > 0.f ? code_of(f, s, inv) : 0;
-                now |= (slot < from ? old & (0xffu << (8 * e)) : (unsigned)(code & 0xff) << (8 * e));
+            for (int e = 0; e < 4; ++e) f[e] = v[u][4 * Square::row(w, e) + Square::column(w, e)];
+            unsigned now = (unsigned)coder.word(f[0], f[1], f[2], f[3], doubtful);
+            unsigned* const at = reinterpret_cast<unsigned*>(codes + p.at(w));
+            if (p.token < from) {
+                const unsigned mask = older(p, w);
+                now = (*at & mask) | (now & ~mask);
             }
             *at = now;
+        }
+    }
+    if (doubtful) {  // (its words once more, one after another)
+#pragma unroll 1
+        for (int n = 0; n < 4 * KC; ++n) {
+            const Square p(tid + 256 * (n >> 2));
+            if (p.token >= to || p.token + 4 <= from) continue;
+            unsigned* const at = reinterpret_cast<unsigned*>(codes + p.at(n & 3));
+            unsigned now = 0;
+#pragma unroll 1
+            for (int e = 0; e < 4; ++e) {
+                const int slot = p.token + Square::row(n & 3, e), d = p.dim + Square::column(n & 3, e);
+                const float f = slot >= from && slot < to && d < c.dim ? rows[(ptrdiff_t)slot * (ptrdiff_t)stride + d] : 0.f;
+                now |= (unsigned)coder.exact(f) << (8 * e);
+            }
+            const unsigned mask = older(p, n & 3);
+            *at = (*at & mask) | (now & ~mask);
         }
     }
     if (tid == 0) *scale = s;

@@ -108,6 +108,19 @@ __device__ __forceinline__ float finite_size(float x) {
     const float a = __builtin_fabsf(x);
     return a < __builtin_inff() ? a : 0.f;
 }
+// The largest finite size of N values: compared as integers, which order sizes as floats do and have what is not finite above all others,
+// so that a value costs a mask and half a comparison; where something is not finite, once more by finite_size.
+template <int N>
+__device__ __forceinline__ float largest_size(const float (&x)[N]) {
+    unsigned most = 0;
+#pragma unroll
+    for (int e = 0; e < N; ++e) most = max(most, __float_as_uint(x[e]) & 0x7fffffffu);
+    if (most < 0x7f800000u) return __uint_as_float(most);
+    float finite = 0.f;
+#pragma unroll
+    for (int e = 0; e < N; ++e) finite = fmaxf(finite, finite_size(x[e]));
+    return finite;
+}
 __device__ __forceinline__ float scale_of(float most) {
     const float s = __fdiv_rn(most, 127.f);
     return s < KV_LEAST_SCALE ? 0.f : s;
@@ -124,6 +137,33 @@ __device__ __forceinline__ int code_of(float x, float s, float inv) {
     const int i = min((int)c, 127);
     return x == x ? (x < 0.f ? -i : i) : 0;
 }
+// The four codes of a word, and whether one of them may be wrong: then code_of has to find them. c = rint(x / s), the quotient off by
+// less than 2^-15, is right where |x - c s| < s / 2; one fused multiply-add has that difference, rounded, and a rounding does not pass s / 2.
+// (Not below s / 2: the middle between two codes, a code that is off by one, an infinity, NaN.) Eight instructions a code with their
+// packing, where code_of is twenty: 23 MB of codes appended in @APPEND@.
+struct Coder {
+    float s, inv, half;
+    __device__ explicit Coder(float scale) : s(scale) {
+        inv = scale > 0.f ? __fdiv_rn(1.f, scale) : 0.f;
+        half = scale > 0.f ? __fmul_rn(scale, 0.5f) : __builtin_inff();
+    }
+    __device__ __forceinline__ int word(float x, float y, float z, float w, bool& doubtful) const {
+        const float v[4] = {x, y, z, w};
+        unsigned c[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const float q = __builtin_rintf(__fmul_rn(v[e], inv));
+            doubtful |= !(__builtin_fabsf(__fmaf_rn(-q, s, v[e])) < half);
+            c[e] = (unsigned)(int)q;
+        }
+        const unsigned low = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400), high = __builtin_amdgcn_perm(c[3], c[2], 0x04000c0c);
+        return (int)(low | high);
+    }
+    __device__ __forceinline__ int exact(float x) const { return s > 0.f ? code_of(x, s, inv) & 0xff : 0; }
+    __device__ __forceinline__ int exact_word(float x, float y, float z, float w) const {
+        return exact(x) | exact(y) << 8 | exact(z) << 16 | exact(w) << 24;
+    }
+};
 
 // kv_cache.hip
 hipError_t run_kv_append(const KvView& c, const KvBatch& b, const float* k, size_t k_stride, const float* v, size_t v_stride, hipStream_t stream);

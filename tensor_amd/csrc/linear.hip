@@ -37,12 +37,9 @@ __device__ __forceinline__ float4 row_quad(const float* __restrict__ row, int d,
     }
     return f;
 }
-__device__ __forceinline__ int codes_of_quad(const float4& f, float s, float inv) {
-    if (!(s > 0.f)) return 0;
-    return (code_of(f.x, s, inv) & 0xff) | ((code_of(f.y, s, inv) & 0xff) << 8) | ((code_of(f.z, s, inv) & 0xff) << 16) | (code_of(f.w, s, inv) << 24);
-}
 __device__ __forceinline__ float most_of_quad(const float4& f) {
-    return fmaxf(fmaxf(finite_size(f.x), finite_size(f.y)), fmaxf(finite_size(f.z), finite_size(f.w)));
+    const float v[4] = {f.x, f.y, f.z, f.w};
+    return largest_size(v);
 }
 
 // A workgroup a row: its largest size, then its codes. 4096 inputs stay in registers, what is behind them is read again.
@@ -56,22 +53,31 @@ __global__ void __launch_bounds__(256) linear_codes_kernel(const float* __restri
     float4 kept[KEPT];
 #pragma unroll
     for (int u = 0; u < KEPT; ++u) kept[u] = row_quad(row, 4 * tid + 1024 * u, in, quads);
-    float most = 0.f;
-#pragma unroll
-    for (int u = 0; u < KEPT; ++u) most = fmaxf(most, most_of_quad(kept[u]));
+    float most = largest_size(reinterpret_cast<const float(&)[4 * KEPT]>(kept));
     for (int d = 4 * tid + 1024 * KEPT; d < in; d += 1024) most = fmaxf(most, most_of_quad(row_quad(row, d, in, quads)));
 #pragma unroll
     for (int m = 32; m; m >>= 1) most = fmaxf(most, __shfl_xor(most, m));
     if ((tid & 63) == 0) most_of[tid >> 6] = most;
     __syncthreads();
     const float s = scale_of(fmaxf(fmaxf(most_of[0], most_of[1]), fmaxf(most_of[2], most_of[3])));
-    const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+    const Coder coder(s);
     if (tid == 0) scale[blockIdx.x] = s;
     int* const to = reinterpret_cast<int*>(codes + (size_t)blockIdx.x * padded);
+    bool doubtful = false;
 #pragma unroll
     for (int u = 0; u < KEPT; ++u)
-        if (4 * tid + 1024 * u < padded) to[tid + 256 * u] = codes_of_quad(kept[u], s, inv);
-    for (int d = 4 * tid + 1024 * KEPT; d < padded; d += 1024) to[d >> 2] = codes_of_quad(row_quad(row, d, in, quads), s, inv);
+        if (4 * tid + 1024 * u < padded) to[tid + 256 * u] = coder.word(kept[u].x, kept[u].y, kept[u].z, kept[u].w, doubtful);
+    for (int d = 4 * tid + 1024 * KEPT; d < padded; d += 1024) {
+        const float4 f = row_quad(row, d, in, quads);
+        to[d >> 2] = coder.word(f.x, f.y, f.z, f.w, doubtful);
+    }
+    if (doubtful) {
+#pragma unroll 1
+        for (int d = 4 * tid; d < padded; d += 1024) {
+            const float4 f = row_quad(row, d, in, quads);
+            to[d >> 2] = coder.exact_word(f.x, f.y, f.z, f.w);
+        }
+    }
 }
 
 struct LinearArgs {
@@ -273,10 +279,14 @@ __global__ void __launch_bounds__(64 * W) linear_rows_kernel(LinearArgs a, const
     for (int r = first; r < count; r += apart) {
         const int src = linear_source(a, t.begin + r);
         const float* const row = x + (size_t)max(src, 0) * x_stride;
-        const float s = scale_of_row(r), inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+        const Coder coder(scale_of_row(r));
         for (int q = q0 + lane; q < q1; q += 64) {
             const int piece = (q >> 2) ^ ((r >> 1) & 7);
-            *reinterpret_cast<int*>(lds + r * row_bytes + piece * 16 + (q & 3) * 4) = codes_of_quad(row_quad(row, 4 * q, in, quads), s, inv);
+            const float4 f = row_quad(row, 4 * q, in, quads);
+            bool doubtful = false;
+            int code = coder.word(f.x, f.y, f.z, f.w, doubtful);
+            if (doubtful) code = coder.exact_word(f.x, f.y, f.z, f.w);
+            *reinterpret_cast<int*>(lds + r * row_bytes + piece * 16 + (q & 3) * 4) = code;
         }
     }
     __syncthreads();
