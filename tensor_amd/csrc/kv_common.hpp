@@ -44,6 +44,7 @@ struct KvSeq {
     int length;        // tokens, with those of the rows
     int first;         // position of its first row (below 0: the batch says more rows than tokens)
     int tile;          // of the sequence (below 0: of none)
+    int all;           // tiles of all sequences (-1: more than 64 of them, not counted)
 };
 
 // The sum over this lane and those below it.
@@ -69,7 +70,7 @@ template <int UNIT, bool BLOCKS, bool LENGTHS>
 __device__ __forceinline__ KvSeq kv_locate(const int32_t* starts, const int32_t* lengths, int n, int limit, int mul, int tile) {
     constexpr int SLACK = BLOCKS ? 2 : 1;
     const int lane = (int)(threadIdx.x & 63);
-    int lo = 0;
+    int lo = 0, all = -1;
     const bool few = n <= 64;
     for (;;) {
         const int step = (n + 63) >> 6, i = lane * step, at = lo + min(i, n - 1);
@@ -80,7 +81,9 @@ __device__ __forceinline__ KvSeq kv_locate(const int32_t* starts, const int32_t*
         if (few) {
             int tiles = BLOCKS ? ((length - 1) >> 6) - ((length - count) >> 6) + 1 : (int)((unsigned)(count * mul + UNIT - 1) / UNIT);
             if (i >= n || count == 0) tiles = 0;
-            base = lanes_below(tiles) - tiles;
+            base = lanes_below(tiles);
+            all = __builtin_amdgcn_readlane(base, 63);
+            base -= tiles;
             const unsigned long long mine = __ballot(tiles > 0 && base <= tile);
             k = mine ? 63 - __builtin_clzll(mine) : 0;
             if (!mine) base = tile + 1;  // (no sequence has rows)
@@ -96,6 +99,7 @@ __device__ __forceinline__ KvSeq kv_locate(const int32_t* starts, const int32_t*
             s.length = __builtin_amdgcn_readlane(length, k);
             s.first = s.length - s.count;
             s.tile = tile - __builtin_amdgcn_readlane(base, k);
+            s.all = all;
             return s;
         }
         lo += k * step;

@@ -93,16 +93,17 @@ struct LinearArgs {
 // Expert and rows of a tile of UNIT rows: [begin, end), empty where the tile is behind its expert's rows.
 struct LinearTile {
     int expert, begin, end;
+    int all;  // tiles of all experts (-1: not counted)
 };
 template <int UNIT>
 __device__ __forceinline__ LinearTile linear_tile(const LinearArgs& a, int tile) {
     LinearTile t;
     if (!a.starts) {
-        t.expert = 0, t.begin = tile * UNIT, t.end = min(t.begin + UNIT, a.rows);
+        t.expert = 0, t.begin = min(tile * UNIT, a.rows), t.end = min(t.begin + UNIT, a.rows), t.all = (a.rows + UNIT - 1) / UNIT;
         return t;
     }
     const KvSeq s = kv_locate<UNIT, false, false>(a.starts, nullptr, a.w.experts, a.rows, 1, tile);
-    t.expert = s.index;
+    t.expert = s.index, t.all = s.all;
     const int to = s.begin + s.count;
     t.begin = s.tile < 0 ? to : min(s.begin + s.tile * UNIT, to);
     t.end = min(t.begin + UNIT, to);
@@ -323,15 +324,16 @@ __global__ void __launch_bounds__(64 * W) linear_rows_kernel(LinearArgs a, const
 // wave of the workgroup reads, straight into registers, a stage of 128 inputs ahead; the rows' codes, which all four waves read, go
 // through LDS, in lane order too (a 16-byte piece of a row is a lane's). A stage is 8 NT RT matrix instructions a wave against 2 RT KB
 // from LDS and 2 NT KB from memory: with 4 and 8 that is 64 and 32 bytes a cycle of a compute unit's 128 and 64.
+template <int NT, int RT>
+struct LinearRing {
+    v4i rows[3][RT][2][64];
+};
 template <int NT, int RT, int END>
-__global__ void __launch_bounds__(256, 2) linear_many_kernel(LinearArgs a) {
+__device__ __forceinline__ void linear_many(const LinearArgs& a, const LinearTile& t, int first_tile, void* lds) {
     constexpr int MINE = RT / 4;  // tiles of 16 rows that a wave brings in
-    __shared__ v4i rows[3][RT][2][64];
+    auto& rows = reinterpret_cast<LinearRing<NT, RT>*>(lds)->rows;
     const int lane = (int)threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x >> 6);
-    const unsigned n_blocks = (unsigned)(a.w.tiles + 4 * NT - 1) / (4 * NT);
-    const LinearTile t = linear_tile<16 * RT>(a, (int)(blockIdx.x / n_blocks));
-    if (t.begin >= t.end) return;
-    const int tile0 = ((int)(blockIdx.x % n_blocks) * 4 + wave) * NT, steps = a.w.steps;
+    const int tile0 = first_tile + wave * NT, steps = a.w.steps;
     const size_t row_bytes = linear_row_bytes(steps);
     const int8_t* w[NT];  // (the same for every lane: the lane's share is a 32-bit offset to it)
 #pragma unroll
@@ -425,6 +427,30 @@ __global__ void __launch_bounds__(256, 2) linear_many_kernel(LinearArgs a) {
     else finish(false);
 }
 
+// Two workgroups of 64 x 128 results a wave fill a compute unit. Where a grid of them is a few more than whole rounds, those few are cut in
+// four each: one of them by itself takes 1.55 us a stage, a quarter 0.62. 4096 x 4096 with codes, 512 workgroups 94 us, 544: 99 (uncut
+// 113), 608: 109 (114), 640 would be 119 (115); 1056: 174 (189). (More than 64 experts: their tiles are not counted, and not cut.)
+constexpr int LINEAR_PLACES = 512, LINEAR_CUT = 96;
+template <int NT, int RT, int END>
+__global__ void __launch_bounds__(256, 2) linear_many_kernel(LinearArgs a) {
+    __shared__ LinearRing<NT, RT> lds;
+    const int n_blocks = (a.w.tiles + 4 * NT - 1) / (4 * NT), group = (int)blockIdx.x;
+    LinearTile t = linear_tile<16 * RT>(a, group / n_blocks);
+    if constexpr (RT == 8) {
+        const int all = t.all * n_blocks, over = all % LINEAR_PLACES;
+        if (all >= LINEAR_PLACES && over <= LINEAR_CUT && group >= all - over) {
+            const int part = group - (all - over), cut = all - over + (part >> 2);
+            if (cut >= all) return;
+            t = linear_tile<16 * RT>(a, cut / n_blocks);
+            t.begin = min(t.begin + (part & 2) * 32, t.end);
+            t.end = min(t.begin + 64, t.end);
+            if (t.begin < t.end) linear_many<NT / 2, RT / 2, END>(a, t, (cut % n_blocks * 2 + (part & 1)) * 2 * NT, &lds);
+            return;
+        }
+    }
+    if (t.begin < t.end) linear_many<NT, RT, END>(a, t, group % n_blocks * 4 * NT, &lds);
+}
+
 #define OHIP_LINEAR_END(CALL)                                  \
     switch (linear_end(a.w)) {                                 \
     case LINEAR_GATED: CALL(LINEAR_GATED); break;              \
@@ -436,7 +462,8 @@ __global__ void __launch_bounds__(256, 2) linear_many_kernel(LinearArgs a) {
     }
 static size_t few_groups(const LinearView& w, const LinearRows& r) { return (size_t)(w.tiles / (w.gated ? 2 : 1)) * linear_row_tiles(w, r, 16); }
 static size_t many_groups(const LinearView& w, const LinearRows& r, int nt, int rt) {
-    return (size_t)((w.tiles + 4 * nt - 1) / (4 * nt)) * linear_row_tiles(w, r, 16 * rt);
+    const size_t n = (size_t)((w.tiles + 4 * nt - 1) / (4 * nt)) * linear_row_tiles(w, r, 16 * rt);
+    return rt == 8 && n >= LINEAR_PLACES ? n + 3 * LINEAR_CUT : n;  // (with the quarters of those that are cut, however many the experts' rows make)
 }
 size_t linear_groups(const LinearView& w, const LinearRows& r) {
     const int k = linear_choice(w, r.rows);

@@ -275,3 +275,38 @@ def test_refusals_of_the_binding(hip):
     layer.close()
     with pytest.raises(capi.HipError):
         layer.forward(x, starts)
+
+
+@pytest.mark.parametrize("experts,counts,k,n,gated", [
+    (1, [128 * 32 + 1], 64, 4096, False),           # 33 x 16 workgroups: 16 behind a round
+    (1, [128 * 37 + 70], 100, 4000, False),         # 96 behind a round, the last with the end of the rows and of the outputs
+    (1, [128 * 38 + 3], 64, 4096, False),           # 112: not cut
+    (1, [128 * 127 + 128], 130, 2056, True),        # gated, two rounds and 128 blocks of 17
+    (5, [1000, 0, 1300, 1, 1930], 192, 4099, False),  # experts of no whole tiles, an odd number of outputs
+    (70, [60] * 70, 64, 2100, False)])              # too many experts for their tiles to be counted
+def test_workgroups_behind_the_last_whole_round(hip, experts, counts, k, n, gated):
+    """The launch of the largest tiles cuts the few that a round of workgroups leaves: the same results as from small tiles, bit by bit."""
+    rng = np.random.default_rng(k + n)
+    w, s, b = weights(rng, experts, n, k)
+    starts, index = route(rng, experts, counts, 300, front=5, behind=4)
+    layer = hip.linear(weight=w, scale=s, bias=b, gated=gated)
+    x, st, ix = hip.to_device(rng.normal(0, 1, (300, k)).astype(np.float32)), dev(hip, starts), dev(hip, index)
+    results = []
+    for kind in (1, 3):
+        layer.set_kernel(kind)
+        out = hip.torch.full((len(index), layer.out_features), 7.5, device=hip.device)
+        layer.forward(x, st, ix, out=out)
+        results.append(out)
+        whole = hip.torch.full((sum(counts), layer.out_features), 7.5, device=hip.device)
+        if experts == 1:  # (without `starts` or an index)
+            layer.forward(x[ix[5:5 + sum(counts)].long()], out=whole)
+            assert hip.torch.equal(whole, out[5:5 + sum(counts)])
+    layer.close()
+    assert hip.torch.equal(results[0], results[1])
+    assert hip.torch.all(results[1][:5] == 7.5) and hip.torch.all(results[1][-4:] == 7.5)
+    few = np.r_[5:20, 5 + sum(counts) - 20:5 + sum(counts)]
+    experts_of = np.searchsorted(starts, few, side="right") - 1
+    xn, got = x.cpu().numpy(), results[1].cpu().numpy()
+    for e in set(experts_of.tolist()):
+        rows = few[experts_of == e]
+        check_close(got[rows], *linear(xn, w[e:e + 1], s[e:e + 1], b[e:e + 1], got[rows], index=index[rows], gated=gated))
