@@ -24,6 +24,33 @@ static LinearCodes linear_codes(const LinearView& w, int x_rows, void* workspace
 __host__ __device__ inline size_t linear_row_bytes(int steps) { return (size_t)(steps + 1) / 2 * 128; }
 size_t linear_workspace_bytes(const LinearView& w, int x_rows) { return ((size_t)x_rows * 4 + 255) / 256 * 256 + (size_t)x_rows * linear_row_bytes(w.steps); }
 
+// Weights into tiles of 16 outputs x 64 inputs, in the order of the matrix instruction's lanes: a thread a piece, 16 inputs of an output
+// (zeros behind the last of either).
+__global__ void __launch_bounds__(256) linear_pack_kernel(const int8_t* __restrict__ weight, int8_t* __restrict__ tiles, size_t pieces, int out, int in,
+                                                          int halves, int half_tiles, int steps) {
+    for (size_t piece = (size_t)blockIdx.x * 256 + threadIdx.x; piece < pieces; piece += (size_t)gridDim.x * 256) {
+        const int lane = (int)(piece & 63);
+        const size_t tile = (piece >> 6) / (unsigned)steps;  // of all experts, the halves in turn
+        const int step = (int)((piece >> 6) % (unsigned)steps), half = (int)(tile % (unsigned)halves);
+        const size_t pair = tile / (unsigned)halves, expert = pair / (unsigned)half_tiles;
+        const int n = (int)(pair % (unsigned)half_tiles) * 16 + (lane & 15), k = step * 64 + (lane >> 4) * 16;
+        int8_t v[16] __attribute__((aligned(16))) = {};
+        if (n < out) {
+            const int8_t* const from = weight + ((expert * halves + half) * (size_t)out + n) * in;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (k + i < in) v[i] = from[k + i];
+        }
+        *reinterpret_cast<v4i*>(tiles + piece * 16) = *reinterpret_cast<const v4i*>(v);
+    }
+}
+hipError_t run_linear_pack(const int8_t* weight, int8_t* tiles, int experts, int out, int in, int halves) {
+    const int half_tiles = (out + 15) / 16, steps = (in + 63) / 64;
+    const size_t pieces = (size_t)experts * halves * half_tiles * steps * 64;
+    launch(linear_pack_kernel, dim3((unsigned)std::min<size_t>((pieces + 255) / 256, 65536)), dim3(256), 0, nullptr, weight, tiles, pieces, out, in, halves, half_tiles, steps);
+    return hipGetLastError();
+}
+
 // Four inputs of a row from d on; those behind its last are 0.
 __device__ __forceinline__ float4 row_quad(const float* __restrict__ row, int d, int in, bool quads) {
     float4 f = {0.f, 0.f, 0.f, 0.f};

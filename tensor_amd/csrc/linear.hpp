@@ -22,6 +22,8 @@ struct LinearRows {
     int rows;
     float* y;
 };
+// Weights [experts][halves][out][in] into the tiles of LinearView (by the null stream).
+hipError_t run_linear_pack(const int8_t* weight, int8_t* tiles, int experts, int out, int in, int halves);
 size_t linear_workspace_bytes(const LinearView& w, int x_rows);
 int linear_choice(const LinearView& w, int rows);  // otter_hip_linear_kernel_kind
 size_t linear_groups(const LinearView& w, const LinearRows& r);  // workgroups of its launch
