@@ -650,7 +650,7 @@ int otter_hip_kv_read(const otter_hip_kv_cache* cache, const otter_hip_kv_batch*
  * over the sequence's tokens j, with causal j <= position, with window > 0 position - j < window. A row that sees none is 0; a row
  * of q that holds a NaN or an infinity gives NaN. Query head h reads key head h / (q_heads / heads).
  *   q    fp32, a row every q_stride elements, q_heads * head_dim consecutive values; out [n_tokens][q_heads][head_dim]
- *   slopes  device, [q_heads], or NULL
+ *   slopes  device, [q_heads], or NULL; out overlaps neither q nor the workspace
  * The scores are those of q rounded to 22 bits below the row's largest element, all else is fp32. A row's result does not depend on the
  * rows of other sequences, but on how many workgroups its tokens are dealt to, which follows from n_seqs, n_tokens, max_pages and the heads.
  * workspace: otter_hip_kv_attend_workspace_bytes (0 where one workgroup has a row's tokens), 16-byte aligned. */
@@ -688,6 +688,7 @@ int otter_hip_linear_destroy(otter_hip_linear_t* handle);
  *   index   [rows]: the row of x that row r is, any number of times each (outside of x: a row of zeros), or NULL: row r itself
  *   starts  [experts + 1], not decreasing: rows starts[e] .. starts[e+1] - 1 are expert e's; rows of none are left as they were. NULL
  *           with one expert: all rows
+ * y overlaps neither x nor the workspace.
  * workspace: otter_hip_linear_workspace_bytes, 16-byte aligned. */
 size_t otter_hip_linear_workspace_bytes(const otter_hip_linear_t* handle, int x_rows, int rows);
 int otter_hip_linear_forward(const otter_hip_linear_t* handle, const float* x, size_t x_stride, int x_rows, const int32_t* index,

@@ -314,6 +314,11 @@ const char* not_as(const at::Tensor* t, at::ScalarType dt, long device, std::ini
     }
     return nullptr;
 }
+// (a workspace is memory alone: of any type and shape)
+const char* no_workspace(const at::Tensor* t, long device) {
+    if (t && (t->layout() != at::kStrided || !t->is_cuda() || t->get_device() != device)) return "a tensor on the library's GPU expected";
+    return t && !t->is_contiguous() ? "not contiguous" : nullptr;
+}
 PyObject* refuse(const char* call, const char* what, const char* why) {
     PyObject* args = Py_BuildValue("(iN)", OTTER_HIP_ERR_INVALID, PyUnicode_FromFormat("%s: %s: %s", call, what, why));
     if (args) PyErr_SetObject(g_error ? g_error : PyExc_RuntimeError, args);
@@ -409,6 +414,7 @@ PyObject* kv_attend(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
             d.slopes = (const float*)slopes->data_ptr();
         }
         if (out) AS("kv_attend", "out", out, at::kFloat, device, {b->n_tokens, d.q_heads, c->head_dim})
+        if (const char* why = no_workspace(ws, device)) return refuse("kv_attend", "workspace", why);
         const c10::DeviceGuard on(c10::Device(c10::DeviceType::CUDA, (c10::DeviceIndex)device));
         at::Tensor made, made_ws;
         if (!out) out = &(made = device_empty(q->sizes(), at::kFloat, device));
@@ -449,6 +455,7 @@ PyObject* linear_forward(PyObject*, PyObject* const* a, Py_ssize_t nargs) {
         if (out) AS("linear", "out", out, at::kFloat, device, {shape[0], columns})
         if (x->size(0) > INT_MAX || shape[0] > INT_MAX) return refuse("linear", "x", "too many rows");
         const int x_rows = (int)x->size(0), rows = (int)shape[0];
+        if (const char* why = no_workspace(ws, device)) return refuse("linear", "workspace", why);
         const c10::DeviceGuard on(c10::Device(c10::DeviceType::CUDA, (c10::DeviceIndex)device));
         at::Tensor made, made_ws;
         if (!out) out = &(made = device_empty(at::IntArrayRef(shape, 2), at::kFloat, device));

@@ -671,8 +671,8 @@ class KvBatch:
         n = lengths.shape[0]
         lib.check_tensor(starts, i32, (n + 1,), "starts")
         lib.check_tensor(pages, i32, (n, None), "pages")
-        if n_tokens < 0:
-            raise HipError(-2, "kv_batch: negative n_tokens")
+        if not 0 <= n_tokens < 2 ** 31 or pages.shape[1] >= 2 ** 31:
+            raise HipError(-2, "kv_batch: n_tokens and max_pages have to be 0 or more, in 32 bits")
         self.starts, self.lengths, self.pages, self.n_tokens = starts, lengths, pages, int(n_tokens)
         self.args = KvBatchArgs(n, self.n_tokens, pages.shape[1], starts.data_ptr(), lengths.data_ptr(), pages.data_ptr())
         self._bp = C.addressof(self.args)

@@ -2473,6 +2473,7 @@ int otter_hip_linear_create(const otter_hip_linear_desc* desc, const int8_t* wei
             OHIP_CHECK(hipMalloc(&h->w, bytes));
             OHIP_CHECK(run_linear_pack(raw, h->w, d.experts, d.out_features, d.in_features, halves));
             OHIP_CHECK(hipStreamSynchronize(nullptr));
+            t_launched.waited_for(nullptr);
             return OTTER_HIP_OK;
         };
         rc = put((void**)&raw, weight, (size_t)d.experts * halves * d.out_features * d.in_features);

@@ -469,6 +469,27 @@ def test_refusals_of_the_binding(hip):
         hip.kv_batch(*i, -1)
 
 
+def test_refusals_of_workspaces_and_of_sizes_beyond_32_bits(hip):
+    torch = hip.torch
+    cache = hip.kv_cache(1024, 1, 64)
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32, device=hip.device)
+    starts, lengths, pages = i32(0, 1), i32(60000), torch.arange(1024, dtype=torch.int32, device=hip.device)[None]
+    batch = hip.kv_batch(starts, lengths, pages, 1)
+    q = torch.zeros((1, 1, 64), device=hip.device)
+    wide = torch.zeros((1 << 20, 2), device=hip.device)
+    for workspace in (torch.zeros(1 << 20), wide[:, 0], torch.zeros(4, device=hip.device)):
+        with pytest.raises(capi.HipError):
+            cache.attend(batch, q, workspace=workspace)
+    layer = hip.linear(weight=np.ones((16, 64), np.int8), scale=np.ones(16, np.float32))
+    for workspace in (torch.zeros(1 << 20), wide[:, 0], torch.zeros(4, device=hip.device)):
+        with pytest.raises(capi.HipError):
+            layer.forward(wide[:4].reshape(-1, 1).expand(8, 64)[:, :64].contiguous(), workspace=workspace)
+    layer.close()
+    for n in (-1, 2 ** 31, 2 ** 32 + 1):
+        with pytest.raises(capi.HipError):
+            hip.kv_batch(starts, lengths, pages, n)
+
+
 def test_nothing_to_do(hip):
     cache = hip.kv_cache(4, 2, 64)
     none = hip.torch.zeros((0, 2, 64), device=hip.device)
