@@ -18,6 +18,10 @@
 
 namespace ohip {
 
+// tanh(x) / x as a polynomial of x^2, the smallest largest relative error for |x| < 1/2: 2^-26.
+constexpr int TANH_TERMS = 5;
+constexpr double TANH_TERM[TANH_TERMS] = {0.9999999868718333, -0.3333306939402176, 0.13324779317606145, -0.05298607529097958, 0.0171350066330358};
+
 struct AttendArgs {
     KvView c;
     KvBatch b;
@@ -27,6 +31,7 @@ struct AttendArgs {
     int q_heads, group;
     float scale;  // with cap: scale / cap, else scale * log2(e)
     float cap;    // cap * log2(e), 0: none
+    float half[TANH_TERMS];  // cap times the terms of tanh below 1/2
     const float* slopes;
     int causal, window;
     int tiles, splits;
@@ -52,7 +57,7 @@ __device__ __forceinline__ float quad_sum(float x) {
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // tanh. 1 - 2 / (exp(2 x) + 1) loses the bits of a small x, where the series goes on (to x^9 below 1/4, where the next term is under
-// 2^-26 of x; to x^13 below 1/2).
+// 2^-26 of x).
 __device__ __forceinline__ float tanh_of(float x) {
     const float a = __builtin_fabsf(x), y = __fmul_rn(x, x);
     const float big = __fmaf_rn(-2.f, __fdividef(1.f, __fadd_rn(fast_exp2(__fmul_rn(a, 2.f * LOG2E)), 1.f)), 1.f);
@@ -62,14 +67,12 @@ __device__ __forceinline__ float tanh_of(float x) {
     s = __fmaf_rn(__fmul_rn(y, a), s, a);
     return __builtin_copysignf(a < 0.25f ? s : big, x);
 }
-__device__ __forceinline__ float tanh_of_half(float x) {  // |x| < 1/2
-    const float y = __fmul_rn(x, x);
-    float s = __fmaf_rn(y, 21844.f / 6081075.f, -1382.f / 155925.f);
-    s = __fmaf_rn(y, s, 62.f / 2835.f);
-    s = __fmaf_rn(y, s, -17.f / 315.f);
-    s = __fmaf_rn(y, s, 2.f / 15.f);
-    s = __fmaf_rn(y, s, -1.f / 3.f);
-    return __fmaf_rn(__fmul_rn(y, x), s, x);
+// cap * tanh(x) / x for |x| < 1/2, of x * x
+__device__ __forceinline__ float tanh_of_half(float y, const float (&terms)[TANH_TERMS]) {
+    float s = terms[TANH_TERMS - 1];
+#pragma unroll
+    for (int n = TANH_TERMS - 2; n >= 0; --n) s = __fmaf_rn(y, s, terms[n]);
+    return s;
 }
 
 // Three signed digits of four fixed-point numbers (u = number + 0x8080 in the low 24 bits): u's low two bytes less 128, and the third.
@@ -160,18 +163,20 @@ struct Pages {
 struct RowView {
     int lo, hi, p;
     float slope;
+    float rise[4][4];  // slope * distance to the page's last token, below 0, of a lane's scores
 };
 
 // NP pages into a wave's 16 rows. key(page, tile) and value(page, tile): the lane's 16 bytes of a tile; keys_done and values_done: called
-// when the last of them is used. whole: every row sees all of them. Two pages at a time share the conversions of the second product's sums and the rescaling of o, a quarter of the vector
+// when the last of them is used. whole: every row sees all of them; behind: none of their
+// tokens is behind a row. Two pages at a time share the conversions of the second product's sums and the rescaling of o, a quarter of the vector
 // instructions of one: the weights go in as multiples of the pages' value scales, in units of 2^-22 of the largest such product.
 template <int KC, int EXTRA, int NP, typename Key, typename Value, typename KeysDone, typename ValuesDone>
 __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& q, const Key& key, const Value& value, const KeysDone& keys_done,
-                                             const ValuesDone& values_done, const Pages<NP>& at, float factor, float cap, const RowView& row,
-                                             bool whole) {
+                                             const ValuesDone& values_done, const Pages<NP>& at, float factor, const AttendArgs& args, const RowView& row,
+                                             bool whole, bool behind) {
     const int g = (int)(threadIdx.x >> 4) & 3;
-    // scores (log2) are t * unit_of; without cap and slopes the product is left to the subtraction of the maximum
-    float t[NP][4][4], most_of[NP], unit_of[NP];
+    // scores (log2) are t * unit_of + away; without cap and slopes the product is left to the subtraction of the maximum
+    float t[NP][4][4], most_of[NP], unit_of[NP], away = 0.f;
 #pragma unroll
     for (int p = 0; p < NP; ++p) {
         const float unit = __fmul_rn(factor, at.k_scale[p]);
@@ -191,24 +196,42 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
                 t[p][kt][r] = EXTRA == 0 ? x : __fmul_rn(x, unit);
             }
         }
-        if (EXTRA == 1 || (EXTRA == 2 && cap != 0.f)) {
-            // most scores are far below the cap: a third of the instructions for a page where all are below half of it
-            float far = 0.f;
+        if constexpr (EXTRA != 0) {
+            // In a page whose tokens are no further than the rows (`behind`) the distance is that of the page's last token, the same for all,
+            // which joins the maximum, and what a token is in front of it, added with the score's last product. (Relative to the nearest
+            // token the sums are as precise as those of the tokens that count. Over 64 dims there are no registers for it.)
+            static_assert(NP == 1, "one page has one `away`");
+            // last(i, x, f): score i is x * f, less its slope
+            const auto scores = [&](const auto& last) {
+                float (&x)[4][4] = t[p];
+                if (args.cap != 0.f) {
+                    // most scores are far below the cap: a third of the instructions for a page where all are below half of it
+                    float far = 0.f;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) far = fmaxf(far, __builtin_fabsf(t[p][i >> 2][i & 3]));
-            if (__all(far < 0.5f)) {
+                    for (int i = 0; i < 16; ++i) far = fmaxf(far, __builtin_fabsf(x[i >> 2][i & 3]));
+                    if (__all(far < 0.5f)) {
 #pragma unroll
-                for (int i = 0; i < 16; ++i) t[p][i >> 2][i & 3] = __fmul_rn(tanh_of_half(t[p][i >> 2][i & 3]), cap);
+                        for (int i = 0; i < 16; ++i)
+                            x[i >> 2][i & 3] = last(i, x[i >> 2][i & 3], tanh_of_half(__fmul_rn(x[i >> 2][i & 3], x[i >> 2][i & 3]), args.half));
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) x[i >> 2][i & 3] = last(i, tanh_of(x[i >> 2][i & 3]), args.cap);
+                    }
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) x[i >> 2][i & 3] = last(i, x[i >> 2][i & 3], 1.f);
+                }
+            };
+            if constexpr (EXTRA == 1) scores([](int, float x, float f) { return __fmul_rn(x, f); });
+            else if (KC == 1 && behind) {
+                away = __fmul_rn(-row.slope, (float)(row.p - (at.first[p] + KV_BLOCK - 1)));
+                scores([&](int i, float x, float f) { return __fmaf_rn(x, f, row.rise[i >> 2][i & 3]); });
             } else {
-#pragma unroll
-                for (int i = 0; i < 16; ++i) t[p][i >> 2][i & 3] = __fmul_rn(tanh_of(t[p][i >> 2][i & 3]), cap);
+                const float to = (float)(row.p - at.first[p] - 4 * g);
+                scores([&](int i, float x, float f) {
+                    return __fmaf_rn(-row.slope, __builtin_fabsf(__fadd_rn(to, -(float)(16 * (i >> 2) + (i & 3)))), __fmul_rn(x, f));
+                });
             }
-        }
-        if constexpr (EXTRA == 2) {
-            const float away = (float)(row.p - at.first[p] - 4 * g);
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                t[p][i >> 2][i & 3] = __fmaf_rn(-row.slope, __builtin_fabsf(__fadd_rn(away, -(float)(16 * (i >> 2) + (i & 3)))), t[p][i >> 2][i & 3]);
         }
         if (!whole) {
             const int lo = row.lo - at.first[p], hi = row.hi - at.first[p];
@@ -270,9 +293,10 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
             split_digits(u, low, mid, high);
             w[p][2][kt] = low, w[p][1][kt] = mid, w[p][0][kt] = high;
         }
+    if constexpr (EXTRA == 2 && KC == 1) most = __fadd_rn(most, away);
     const float m = fmaxf(s.m, most);
     const float keep = s.m == -__builtin_inff() ? 0.f : fast_exp2(__fadd_rn(s.m, -m));
-    const float take = sees ? fast_exp2(__fadd_rn(most, -m)) : 0.f;
+    const float take = sees && (EXTRA != 2 || most != -__builtin_inff()) ? fast_exp2(__fadd_rn(most, -m)) : 0.f;
     s.m = m;
     s.l = __fmaf_rn(s.l, keep, __fmul_rn(sum, take));
     const float put = __fmul_rn(__fmul_rn(take, 0x1p-22f), unit);
@@ -338,7 +362,7 @@ constexpr int kv_lds_bytes(bool staged, int waves) {
 // faster way only where it leaves room for three workgroups a compute unit and there are as many, by 6 % for 65 to 128 dims (4096 rows on 14
 // thousand tokens: 1.33 ms, 1.45 without, and 1.46 with two buffers in LDS and two workgroups).
 template <int KC, int EXTRA, bool STAGED, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, STAGED ? 3 : 1) kv_attend_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, STAGED || KC == 1 ? 3 : KC <= 3 ? 2 : 1) kv_attend_kernel(AttendArgs a) {
     static_assert(!STAGED || WAVES == 4, "the staging is dealt to four waves");
     __shared__ __attribute__((aligned(16))) unsigned char lds[kv_lds_bytes<KC>(STAGED, WAVES)];
     typedef float JoinedRows[16][64 * KC + 4];
@@ -365,8 +389,15 @@ __global__ void __launch_bounds__(64 * WAVES, STAGED ? 3 : 1) kv_attend_kernel(A
     const int stored = min(s.length, a.b.max_pages * KV_BLOCK);
     const auto sees_to = [&](int p) { return p < 0 ? 0 : a.causal ? min(stored, p + 1) : stored; };
     const auto sees_from = [&](int p) { return a.window > 0 && p >= a.window ? p - a.window + 1 : 0; };
-    RowView view{sees_from(p), sees_to(p), p, 0.f};
-    if constexpr (EXTRA == 2) view.slope = __fmul_rn(a.slopes[q_head], LOG2E);
+    RowView view;
+    view.lo = sees_from(p), view.hi = sees_to(p), view.p = p, view.slope = 0.f;
+    if constexpr (EXTRA == 2) {
+        view.slope = __fmul_rn(a.slopes[q_head], LOG2E);
+        if constexpr (KC == 1)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) view.rise[i >> 2][i & 3] = __fmul_rn(view.slope, (float)(16 * (i >> 2) + 4 * g + (i & 3) - (KV_BLOCK - 1)));
+    }
+    const int first_p = __builtin_amdgcn_readlane(p, 0);
     // what the wave's rows see: rows are in the order of their tokens
     const int first_hi = __builtin_amdgcn_readlane(view.hi, 0), last_hi = __builtin_amdgcn_readlane(view.hi, 15);
     const int first_lo = __builtin_amdgcn_readlane(view.lo, 0), last_lo = __builtin_amdgcn_readlane(view.lo, 15);
@@ -393,43 +424,45 @@ __global__ void __launch_bounds__(64 * WAVES, STAGED ? 3 : 1) kv_attend_kernel(A
     };
     const auto nothing = [] {};
     if (STAGED && shares == 1) {
-        constexpr int NP = 2, TILES = NP * 8 * KC, MINE = TILES / 4;
-        v4i* const buffer = reinterpret_cast<v4i*>(lds);  // [page][4 KC tiles of keys, as many of values][lane]
-        const int p0 = s.first + row0 / a.group, p1 = s.first + (min(row0 + 64, rows) - 1) / a.group;
-        deal(sees_from(p0), sees_to(p1), (int)blockIdx.y, a.splits);
-        if (walk.from < walk.to) {
-            load_rows();
-            v4i mine_of[MINE];
-            Pages<NP> at, next;
-            const auto load = [&](int pg) {
-                const int8_t *kp[NP], *vp[NP];
-                next = pages_at<NP>(a.c, head, walk, pg, kp, vp);
+        if constexpr (STAGED) {
+            constexpr int NP = 2, TILES = NP * 8 * KC, MINE = TILES / 4;
+            v4i* const buffer = reinterpret_cast<v4i*>(lds);  // [page][4 KC tiles of keys, as many of values][lane]
+            const int p0 = s.first + row0 / a.group, p1 = s.first + (min(row0 + 64, rows) - 1) / a.group;
+            deal(sees_from(p0), sees_to(p1), (int)blockIdx.y, a.splits);
+            if (walk.from < walk.to) {
+                load_rows();
+                v4i mine_of[MINE];
+                Pages<NP> at, next;
+                const auto load = [&](int pg) {
+                    const int8_t *kp[NP], *vp[NP];
+                    next = pages_at<NP>(a.c, head, walk, pg, kp, vp);
 #pragma unroll
-                for (int u = 0; u < MINE; ++u) {
-                    const int j = wave * MINE + u, n = j / (8 * KC), of = j % (8 * KC);
-                    const int8_t *const k = n ? kp[1] : kp[0], *const v = n ? vp[1] : vp[0];
-                    mine_of[u] = *reinterpret_cast<const v4i*>((of < 4 * KC ? k + of * 1024 : v + (of - 4 * KC) * 1024) + lane16);
-                }
-            };
-            const auto put = [&] {
+                    for (int u = 0; u < MINE; ++u) {
+                        const int j = wave * MINE + u, n = j / (8 * KC), of = j % (8 * KC);
+                        const int8_t *const k = n ? kp[1] : kp[0], *const v = n ? vp[1] : vp[0];
+                        mine_of[u] = *reinterpret_cast<const v4i*>((of < 4 * KC ? k + of * 1024 : v + (of - 4 * KC) * 1024) + lane16);
+                    }
+                };
+                const auto put = [&] {
 #pragma unroll
-                for (int u = 0; u < MINE; ++u) buffer[(wave * MINE + u) * 64 + lane] = mine_of[u];
-            };
-            load(walk.from);
-            for (int pg = walk.from; pg < walk.to; pg += NP) {
-                at = next;
-                put();
-                if (pg + NP < walk.to) load(pg + NP);
-                // these pages are in LDS (loads from memory stay in flight)
-                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                if (works && pg * KV_BLOCK < last_hi && (pg + NP) * KV_BLOCK > first_lo) {
-                    const bool whole = at.all && (pg + NP) * KV_BLOCK <= first_hi && pg * KV_BLOCK >= last_lo;
-                    const v4i* const from = buffer + lane;
-                    attend_pages<KC, EXTRA, NP>(
-                        run, q, [&](int n, int tile) { return from[(n * 8 * KC + tile) * 64]; },
-                        [&](int n, int tile) { return from[(n * 8 * KC + 4 * KC + tile) * 64]; }, nothing, nothing, at, factor, a.cap, view, whole);
+                    for (int u = 0; u < MINE; ++u) buffer[(wave * MINE + u) * 64 + lane] = mine_of[u];
+                };
+                load(walk.from);
+                for (int pg = walk.from; pg < walk.to; pg += NP) {
+                    at = next;
+                    put();
+                    if (pg + NP < walk.to) load(pg + NP);
+                    // these pages are in LDS (loads from memory stay in flight)
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+                    if (works && pg * KV_BLOCK < last_hi && (pg + NP) * KV_BLOCK > first_lo) {
+                        const bool whole = at.all && (pg + NP) * KV_BLOCK <= first_hi && pg * KV_BLOCK >= last_lo;
+                        const v4i* const from = buffer + lane;
+                        attend_pages<KC, EXTRA, NP>(
+                            run, q, [&](int n, int tile) { return from[(n * 8 * KC + tile) * 64]; },
+                            [&](int n, int tile) { return from[(n * 8 * KC + 4 * KC + tile) * 64]; }, nothing, nothing, at, factor, a, view, whole, false);
+                    }
+                    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // nobody reads them any more
                 }
-                asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // nobody reads them any more
             }
         }
     } else if (works) {
@@ -450,7 +483,7 @@ __global__ void __launch_bounds__(64 * WAVES, STAGED ? 3 : 1) kv_attend_kernel(A
                 const bool whole = at.all && (pg + 1) * KV_BLOCK <= first_hi && pg * KV_BLOCK >= last_lo;
                 attend_pages<KC, EXTRA, 1>(
                     run, q, [&](int, int tile) { return keys[tile]; }, [&](int, int tile) { return values[tile]; }, keys_done, values_done, at, factor,
-                    a.cap, view, whole);
+                    a, view, whole, (pg + 1) * KV_BLOCK <= first_p + 1);
             };
             int pg = walk.from;
             for (; pg + 1 < walk.to; ++pg) {
@@ -633,6 +666,7 @@ hipError_t run_kv_attend(const KvView& c, const KvBatch& b, const float* q, size
     a.c = c, a.b = b, a.q = q, a.q_stride = q_stride, a.out = out, a.q_heads = q_heads, a.group = q_heads / c.heads;
     a.scale = cap != 0.f ? scale / cap : scale * LOG2E;
     a.cap = cap * LOG2E;
+    for (int n = 0; n < TANH_TERMS; ++n) a.half[n] = (float)((double)a.cap * TANH_TERM[n]);
     a.slopes = slopes, a.causal = causal, a.window = window;
     a.tiles = kv_attend_tiles(b.n_tokens, b.n_seqs, a.group), a.splits = splits;
     const size_t rows = (size_t)b.n_tokens * q_heads;
