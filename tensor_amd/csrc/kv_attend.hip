@@ -22,6 +22,11 @@ namespace ohip {
 constexpr int TANH_TERMS = 5;
 constexpr double TANH_TERM[TANH_TERMS] = {0.9999999868718333, -0.3333306939402176, 0.13324779317606145, -0.05298607529097958, 0.0171350066330358};
 
+struct Cap {
+    float cap;               // cap * log2(e), 0: none
+    float half[TANH_TERMS];  // that times the terms of tanh below 1/2
+};
+
 struct AttendArgs {
     KvView c;
     KvBatch b;
@@ -30,8 +35,7 @@ struct AttendArgs {
     float* out;
     int q_heads, group;
     float scale;  // with cap: scale / cap, else scale * log2(e)
-    float cap;    // cap * log2(e), 0: none
-    float half[TANH_TERMS];  // cap times the terms of tanh below 1/2
+    Cap cap;
     const float* slopes;
     int causal, window;
     int tiles, splits;
@@ -56,23 +60,21 @@ __device__ __forceinline__ float quad_sum(float x) {
 }
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// tanh. 1 - 2 / (exp(2 x) + 1) loses the bits of a small x, where the series goes on (to x^9 below 1/4, where the next term is under
-// 2^-26 of x).
+// times * tanh(x) / x for |x| < 1/2, of x * x; terms: TANH_TERM times that
+template <typename Terms>
+__device__ __forceinline__ float tanh_of_half(float y, const Terms& terms) {
+    float s = (float)terms[TANH_TERMS - 1];
+#pragma unroll
+    for (int n = TANH_TERMS - 2; n >= 0; --n) s = __fmaf_rn(y, s, (float)terms[n]);
+    return s;
+}
+// tanh. 1 - 2 / (exp(2 x) + 1) loses the bits of a small x, where the polynomial is taken. (The reciprocal is that of the hardware, off by
+// one unit in the last place at most: a division is ten instructions, a third of all here.)
 __device__ __forceinline__ float tanh_of(float x) {
     const float a = __builtin_fabsf(x), y = __fmul_rn(x, x);
-    const float big = __fmaf_rn(-2.f, __fdividef(1.f, __fadd_rn(fast_exp2(__fmul_rn(a, 2.f * LOG2E)), 1.f)), 1.f);
-    float s = __fmaf_rn(y, 62.f / 2835.f, -17.f / 315.f);
-    s = __fmaf_rn(y, s, 2.f / 15.f);
-    s = __fmaf_rn(y, s, -1.f / 3.f);
-    s = __fmaf_rn(__fmul_rn(y, a), s, a);
-    return __builtin_copysignf(a < 0.25f ? s : big, x);
-}
-// cap * tanh(x) / x for |x| < 1/2, of x * x
-__device__ __forceinline__ float tanh_of_half(float y, const float (&terms)[TANH_TERMS]) {
-    float s = terms[TANH_TERMS - 1];
-#pragma unroll
-    for (int n = TANH_TERMS - 2; n >= 0; --n) s = __fmaf_rn(y, s, terms[n]);
-    return s;
+    const float big = __fmaf_rn(-2.f, __builtin_amdgcn_rcpf(__fadd_rn(fast_exp2(__fmul_rn(a, 2.f * LOG2E)), 1.f)), 1.f);
+    const float small = __fmul_rn(a, tanh_of_half(y, TANH_TERM));
+    return __builtin_copysignf(a < 0.5f ? small : big, x);
 }
 
 // Three signed digits of four fixed-point numbers (u = number + 0x8080 in the low 24 bits): u's low two bytes less 128, and the third.
@@ -172,7 +174,7 @@ struct RowView {
 // instructions of one: the weights go in as multiples of the pages' value scales, in units of 2^-22 of the largest such product.
 template <int KC, int EXTRA, int NP, typename Key, typename Value, typename KeysDone, typename ValuesDone>
 __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& q, const Key& key, const Value& value, const KeysDone& keys_done,
-                                             const ValuesDone& values_done, const Pages<NP>& at, float factor, const AttendArgs& args, const RowView& row,
+                                             const ValuesDone& values_done, const Pages<NP>& at, float factor, const Cap& cap, const RowView& row,
                                              bool whole, bool behind) {
     const int g = (int)(threadIdx.x >> 4) & 3;
     // scores (log2) are t * unit_of + away; without cap and slopes the product is left to the subtraction of the maximum
@@ -192,19 +194,20 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
             }
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                float x = join_digits(a[0][r], a[1][r], a[2][r]);
-                t[p][kt][r] = EXTRA == 0 ? x : __fmul_rn(x, unit);
+                const float x = join_digits(a[0][r], a[1][r], a[2][r]);
+                t[p][kt][r] = EXTRA == 0 ? x : __fmul_rn(x, unit);  // (with a cap too here, in the shadow of the products)
             }
         }
         if constexpr (EXTRA != 0) {
             // In a page whose tokens are no further than the rows (`behind`) the distance is that of the page's last token, the same for all,
             // which joins the maximum, and what a token is in front of it, added with the score's last product. (Relative to the nearest
-            // token the sums are as precise as those of the tokens that count. Over 64 dims there are no registers for it.)
+            // token the sums are as precise as those of the tokens that count. Over 64 dims there are no registers for it, and without a cap
+            // it is no faster.)
             static_assert(NP == 1, "one page has one `away`");
             // last(i, x, f): score i is x * f, less its slope
             const auto scores = [&](const auto& last) {
                 float (&x)[4][4] = t[p];
-                if (args.cap != 0.f) {
+                if (EXTRA == 1 || cap.cap != 0.f) {
                     // most scores are far below the cap: a third of the instructions for a page where all are below half of it
                     float far = 0.f;
 #pragma unroll
@@ -212,10 +215,10 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
                     if (__all(far < 0.5f)) {
 #pragma unroll
                         for (int i = 0; i < 16; ++i)
-                            x[i >> 2][i & 3] = last(i, x[i >> 2][i & 3], tanh_of_half(__fmul_rn(x[i >> 2][i & 3], x[i >> 2][i & 3]), args.half));
+                            x[i >> 2][i & 3] = last(i, x[i >> 2][i & 3], tanh_of_half(__fmul_rn(x[i >> 2][i & 3], x[i >> 2][i & 3]), cap.half));
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) x[i >> 2][i & 3] = last(i, tanh_of(x[i >> 2][i & 3]), args.cap);
+                        for (int i = 0; i < 16; ++i) x[i >> 2][i & 3] = last(i, tanh_of(x[i >> 2][i & 3]), cap.cap);
                     }
                 } else {
 #pragma unroll
@@ -223,7 +226,7 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
                 }
             };
             if constexpr (EXTRA == 1) scores([](int, float x, float f) { return __fmul_rn(x, f); });
-            else if (KC == 1 && behind) {
+            else if (KC == 1 && behind && cap.cap != 0.f) {
                 away = __fmul_rn(-row.slope, (float)(row.p - (at.first[p] + KV_BLOCK - 1)));
                 scores([&](int i, float x, float f) { return __fmaf_rn(x, f, row.rise[i >> 2][i & 3]); });
             } else {
@@ -262,7 +265,7 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
 #pragma unroll
         for (int p = 0; p < NP; ++p) unit = fmaxf(unit, __fmul_rn(fast_exp2(__fadd_rn(most_of[p], -base)), at.v_scale[p]));
         // (finite whatever the scales: a page that the row does not see may have one that is far larger)
-        const float per = unit > 0.f ? fminf(__fdividef(0x1p22f, unit), 0x1p124f) : 0.f;
+        const float per = unit > 0.f ? fminf(__fmul_rn(__builtin_amdgcn_rcpf(unit), 0x1p22f), 0x1p124f) : 0.f;
 #pragma unroll
         for (int p = 0; p < NP; ++p) times[p] = fminf(__fmul_rn(at.v_scale[p], per), 0x1p126f);
     }
@@ -362,7 +365,7 @@ constexpr int kv_lds_bytes(bool staged, int waves) {
 // faster way only where it leaves room for three workgroups a compute unit and there are as many, by 6 % for 65 to 128 dims (4096 rows on 14
 // thousand tokens: 1.33 ms, 1.45 without, and 1.46 with two buffers in LDS and two workgroups).
 template <int KC, int EXTRA, bool STAGED, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, STAGED || KC == 1 ? 3 : KC <= 3 ? 2 : 1) kv_attend_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, STAGED ? 3 : EXTRA < 2 ? 1 : KC == 1 ? 3 : KC <= 3 ? 2 : 1) kv_attend_kernel(AttendArgs a) {
     static_assert(!STAGED || WAVES == 4, "the staging is dealt to four waves");
     __shared__ __attribute__((aligned(16))) unsigned char lds[kv_lds_bytes<KC>(STAGED, WAVES)];
     typedef float JoinedRows[16][64 * KC + 4];
@@ -398,6 +401,12 @@ __global__ void __launch_bounds__(64 * WAVES, STAGED || KC == 1 ? 3 : KC <= 3 ? 
             for (int i = 0; i < 16; ++i) view.rise[i >> 2][i & 3] = __fmul_rn(view.slope, (float)(16 * (i >> 2) + 4 * g + (i & 3) - (KV_BLOCK - 1)));
     }
     const int first_p = __builtin_amdgcn_readlane(p, 0);
+    Cap cap = a.cap;
+    if constexpr (EXTRA != 0) {  // (held in registers: left alone the compiler loads them again for every page, and waits)
+        asm volatile("" : "+s"(cap.cap));
+#pragma unroll
+        for (int n = 0; n < TANH_TERMS; ++n) asm volatile("" : "+s"(cap.half[n]));
+    }
     // what the wave's rows see: rows are in the order of their tokens
     const int first_hi = __builtin_amdgcn_readlane(view.hi, 0), last_hi = __builtin_amdgcn_readlane(view.hi, 15);
     const int first_lo = __builtin_amdgcn_readlane(view.lo, 0), last_lo = __builtin_amdgcn_readlane(view.lo, 15);
@@ -459,7 +468,7 @@ __global__ void __launch_bounds__(64 * WAVES, STAGED || KC == 1 ? 3 : KC <= 3 ? 
                         const v4i* const from = buffer + lane;
                         attend_pages<KC, EXTRA, NP>(
                             run, q, [&](int n, int tile) { return from[(n * 8 * KC + tile) * 64]; },
-                            [&](int n, int tile) { return from[(n * 8 * KC + 4 * KC + tile) * 64]; }, nothing, nothing, at, factor, a, view, whole, false);
+                            [&](int n, int tile) { return from[(n * 8 * KC + 4 * KC + tile) * 64]; }, nothing, nothing, at, factor, cap, view, whole, false);
                     }
                     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // nobody reads them any more
                 }
@@ -483,7 +492,7 @@ __global__ void __launch_bounds__(64 * WAVES, STAGED || KC == 1 ? 3 : KC <= 3 ? 
                 const bool whole = at.all && (pg + 1) * KV_BLOCK <= first_hi && pg * KV_BLOCK >= last_lo;
                 attend_pages<KC, EXTRA, 1>(
                     run, q, [&](int, int tile) { return keys[tile]; }, [&](int, int tile) { return values[tile]; }, keys_done, values_done, at, factor,
-                    a, view, whole, (pg + 1) * KV_BLOCK <= first_p + 1);
+                    cap, view, whole, (pg + 1) * KV_BLOCK <= first_p + 1);
             };
             int pg = walk.from;
             for (; pg + 1 < walk.to; ++pg) {
@@ -645,7 +654,7 @@ int kv_attend_tiles(int n_tokens, int n_seqs, int group) { return (int)((size_t)
 template <int KC, int WAVES>
 static void launch_attend(const AttendArgs& a, dim3 grid, hipStream_t stream) {
     if (a.slopes) launch(kv_attend_kernel<KC, 2, false, WAVES>, grid, dim3(64 * WAVES), 0, stream, a);
-    else if (a.cap != 0.f) launch(kv_attend_kernel<KC, 1, false, WAVES>, grid, dim3(64 * WAVES), 0, stream, a);
+    else if (a.cap.cap != 0.f) launch(kv_attend_kernel<KC, 1, false, WAVES>, grid, dim3(64 * WAVES), 0, stream, a);
     else launch(kv_attend_kernel<KC, 0, false, WAVES>, grid, dim3(64 * WAVES), 0, stream, a);
 }
 template <int KC>
@@ -665,8 +674,8 @@ hipError_t run_kv_attend(const KvView& c, const KvBatch& b, const float* q, size
     AttendArgs a;
     a.c = c, a.b = b, a.q = q, a.q_stride = q_stride, a.out = out, a.q_heads = q_heads, a.group = q_heads / c.heads;
     a.scale = cap != 0.f ? scale / cap : scale * LOG2E;
-    a.cap = cap * LOG2E;
-    for (int n = 0; n < TANH_TERMS; ++n) a.half[n] = (float)((double)a.cap * TANH_TERM[n]);
+    a.cap.cap = cap * LOG2E;
+    for (int n = 0; n < TANH_TERMS; ++n) a.cap.half[n] = (float)((double)a.cap.cap * TANH_TERM[n]);
     a.slopes = slopes, a.causal = causal, a.window = window;
     a.tiles = kv_attend_tiles(b.n_tokens, b.n_seqs, a.group), a.splits = splits;
     const size_t rows = (size_t)b.n_tokens * q_heads;

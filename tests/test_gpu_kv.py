@@ -172,6 +172,31 @@ def test_attend_options(hip, kw, dim):
     s.check_attend(s.now, s.normal(s.now, 1, 6)[0], **kw)
 
 
+@pytest.mark.parametrize("kw", [dict(), dict(causal=False), dict(cap=4.0), dict(cap=60.0, window=200), dict(cap=8.0, causal=False)])
+@pytest.mark.parametrize("dim", [40, 64, 128])
+def test_slopes_of_every_kind(hip, dim, kw):
+    """None, slight and steep ones, such as grow with the distance, on pages in front of the rows, around them and behind them."""
+    rng = np.random.default_rng(dim)
+    s = Setup(hip, rng, 2, dim, [(600, 70), (0, 300), (63, 1), (129, 1), (448, 16)])
+    s.append(s.now, *s.normal(s.now, 2))
+    slopes = np.array([0, 0.001, 0.7, 3.0, -0.02, 0.25], np.float32)
+    s.check_attend(s.now, s.normal(s.now, 1, 6)[0], slopes=slopes, **kw)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+def test_slopes_beyond_all_measure(hip, dim):
+    """A row of them is its own value: every other weight is exp of a million and more below 0."""
+    s = Setup(hip, np.random.default_rng(3), 1, dim, [(600, 70), (0, 200), (700, 1)])
+    k, v = s.normal(s.now, 2)
+    s.append(s.now, k, v)
+    q = hip.to_device(s.normal(s.now, 1, 4)[0])
+    own = s.cache.read(s.now[3])[1].cpu().numpy()
+    for cap in (0.0, 5.0):
+        got = s.cache.attend(s.now[3], q, cap=cap, slopes=hip.to_device(np.array([1e6, 1e30, 1e37, 2e38], np.float32))).cpu().numpy()
+        # the weight is 1 exactly; the codes' products with it are exact, and scaled by 32-bit numbers, four roundings of 2^-24
+        np.testing.assert_allclose(got, np.broadcast_to(own, got.shape), rtol=2.0 ** -21, atol=0)
+
+
 @pytest.mark.parametrize("dim", [64, 128, 192, 200])
 @pytest.mark.parametrize("lengths", [[(2000, 1)], [(3999, 1), (10, 1), (0, 0), (1000, 1)], [(1500, 9)], [(0, 700), (1300, 1)], [(9000, 1)],
                                      [(70, 1), (7000, 2), (0, 1)], [(5000, 40)]])
