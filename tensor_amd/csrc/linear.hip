@@ -439,15 +439,17 @@ __device__ __forceinline__ void linear_many(const LinearArgs& a, const LinearTil
         xs[r] = src < 0 ? 0.f : a.scale[src];
     }
     const auto finish = [&](bool quads) {
+        LinearOut o[NT];
 #pragma unroll
-        for (int n = 0; n < NT; n += G) {
-            if (tile0 + n >= a.w.tiles) break;
-            const LinearOut o = linear_out(a, t.expert, tile0 + n), o_up = linear_out(a, t.expert, tile0 + n + G - 1);
+        for (int n = 0; n < NT; ++n) o[n] = linear_out(a, t.expert, min(tile0 + n, a.w.tiles - 1));
+        // (the pieces of a row one behind the other: stores that pass the caches are written by whole lines then)
 #pragma unroll
-            for (int r = 0; r < RT; ++r) {
-                const int row = t.begin + r * 16 + (lane & 15);
-                if (row < t.end) linear_store<END>(a, row, xs[r], (tile0 + n) / G, acc[n][r], acc[n + G - 1][r], o, o_up, quads);
-            }
+        for (int r = 0; r < RT; ++r) {
+            const int row = t.begin + r * 16 + (lane & 15);
+            if (row >= t.end) continue;
+#pragma unroll
+            for (int n = 0; n < NT; n += G)
+                if (tile0 + n < a.w.tiles) linear_store<END>(a, row, xs[r], (tile0 + n) / G, acc[n][r], acc[n + G - 1][r], o[n], o[n + G - 1], quads);
         }
     };
     if (linear_quads(a)) finish(true);
