@@ -202,7 +202,7 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
             // In a page whose tokens are no further than the rows (`behind`) the distance is that of the page's last token, the same for all,
             // which joins the maximum, and what a token is in front of it, added with the score's last product. (Relative to the nearest
             // token the sums are as precise as those of the tokens that count. Over 64 dims there are no registers for it, and without a cap
-            // it is no faster.)
+            // it is no faster. Six prompts of up to 1900 tokens, cap, slopes, window 512, 16 heads of 64: 56.3 -> 52.2 us with the cap's polynomial.)
             static_assert(NP == 1, "one page has one `away`");
             // last(i, x, f): score i is x * f, less its slope
             const auto scores = [&](const auto& last) {

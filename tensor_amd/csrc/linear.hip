@@ -442,7 +442,7 @@ __device__ __forceinline__ void linear_many(const LinearArgs& a, const LinearTil
         LinearOut o[NT];
 #pragma unroll
         for (int n = 0; n < NT; ++n) o[n] = linear_out(a, t.expert, min(tile0 + n, a.w.tiles - 1));
-        // (the pieces of a row one behind the other: stores that pass the caches are written by whole lines then)
+        // (the pieces of a row one behind the other: stores that pass the caches fill lines sooner. 8192 rows of 4096 x 4000 172.6 -> 170.0 us)
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
             const int row = t.begin + r * 16 + (lane & 15);
@@ -457,8 +457,9 @@ __device__ __forceinline__ void linear_many(const LinearArgs& a, const LinearTil
 }
 
 // Two workgroups of 64 x 128 results a wave fill a compute unit. Where a grid of them is a few more than whole rounds, those few are cut in
-// four each: one of them by itself takes 1.55 us a stage, a quarter 0.62. 4096 x 4096 with codes, 512 workgroups 94 us, 544: 99 (uncut
-// 113), 608: 109 (114), 640 would be 119 (115); 1056: 174 (189). (More than 64 experts: their tiles are not counted, and not cut.)
+// four each: one of them by itself takes 1.55 us a stage, a quarter 0.62. 4096 x 4096 with codes: 512 workgroups 85 us, 544: 93, 608: 107,
+// 1056: 175. (Uncut, when these took 94, 99, 109 and 174: 544 113, 608 114, 640 115, 1056 189; and 640 cut 119. More than 64 experts: their
+// tiles are not counted, and not cut.)
 constexpr int LINEAR_PLACES = 512, LINEAR_CUT = 96;
 template <int NT, int RT, int END>
 __global__ void __launch_bounds__(256, 2) linear_many_kernel(LinearArgs a) {
@@ -531,8 +532,8 @@ static void launch_many(const LinearArgs& a, const LinearRows& r, hipStream_t st
 // rows, 1 to 64 experts; microseconds without the codes): 1 % over the fastest of the four on the mean, 18 % at most. The one for few rows
 // reads weights and rows from the caches at 8 TB/s, 16 x 16 results at a time, but waits 1.2 for every 32 steps. The others take `each`
 // for a stage of a workgroup by itself and `busy` where every compute unit has one, n times that for n: 64 x 128 results a wave are
-// the least traffic, 32 x 64 start the soonest. 4096 x 4096 weights with codes: 128 rows 22 us (few: 26), 512 rows 26.0 (64 x 64: 30.6),
-// 2048 rows 56.2 (32 x 64: 72.6), 8192 rows 193 (64 x 64: 216).
+// the least traffic, 32 x 64 start the soonest. 4096 x 4096 weights with codes: 128 rows 22 us (few: 25), 512 rows 24.1 (64 x 64: 28.2),
+// 2048 rows 49.9 (32 x 64: 66.4), 8192 rows 163 (64 x 64: 192).
 int linear_choice(const LinearView& w, int rows) {
     const bool fits = rows_lds(w, rows) <= 65536;
     if (w.force >= 0) return w.force == 4 && !fits ? 0 : w.force;
