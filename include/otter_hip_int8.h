@@ -651,7 +651,7 @@ int otter_hip_kv_read(const otter_hip_kv_cache* cache, const otter_hip_kv_batch*
  * of q that holds a NaN or an infinity gives NaN. Query head h reads key head h / (q_heads / heads).
  *   q    fp32, a row every q_stride elements, q_heads * head_dim consecutive values; out [n_tokens][q_heads][head_dim]
  *   slopes  device, [q_heads], or NULL; out overlaps neither q nor the workspace
- * The scores are those of q rounded to 22 bits below the row's largest element, all else is fp32. A row's result does not depend on the
+ * The scores are those of q rounded to 23 bits below the row's largest element, all else is fp32. A row's result does not depend on the
  * rows of other sequences, but on how many workgroups its tokens are dealt to, which follows from n_seqs, n_tokens, max_pages and the heads.
  * workspace: otter_hip_kv_attend_workspace_bytes (0 where one workgroup has a row's tokens), 16-byte aligned. */
 typedef struct otter_hip_kv_attend_desc {

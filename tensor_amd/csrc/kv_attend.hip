@@ -4,9 +4,9 @@
 //   o   = sum_j exp(t_j - m) v_j / sum_j exp(t_j - m)
 //
 // Both products run on the int8 matrix cores, on the cache's bytes as they are. The float operands go in as fixed point of three
-// 8-bit digits: a query row in units of 2^-21 of its largest element's binade, the weights exp(t_j - m) in units of 2^-22 of the
-// largest weight that the row has in the page. Digit products and their sums are exact in 32 bits, so a score is off by what
-// rounding q to 22 bits makes of it, and a page's share of o by 2^-23 of the page's largest weight for each token: both are of the
+// 8-bit digits: a query row in units of 2^-22 of its largest element's binade, the weights exp(t_j - m) in units of 1 / WEIGHT_UNITS
+// of the largest weight that the row has in the page. Digit products and their sums are exact in 32 bits, so a score is off by what
+// rounding q to 23 bits makes of it, and a page's share of o by 2^-24 of the page's largest weight for each token: both are of the
 // size that sums in 32-bit floats have. (Half floats would need a second operand for the bits behind the 11th, and the bytes of
 // the cache converted for every row tile: two products at half the rate and five vector instructions for four bytes, against three
 // products at the full rate on bytes that are only loaded.)
@@ -41,6 +41,9 @@ struct AttendArgs {
     int tiles, splits;
     float *part_o, *part_ml;  // of a split: [split][row][dim], [split][row][2] with row = token * q_heads + head
 };
+
+// What a weight of 1 is as a whole number: a little below what three signed digits hold and, with the 0x8080 that makes them, below 2^23.
+constexpr float WEIGHT_UNITS = 8350000.f;
 
 constexpr float LOG2E = 1.44269504088896340736f;
 
@@ -128,11 +131,12 @@ __device__ __forceinline__ void load_queries(Queries<KC>& q, const float* __rest
     }
     most = quad_max(odd ? __builtin_inff() : most);
     odd = !(most < __builtin_inff());
-    // units of 2^(e - 21), most in [2^e, 2^(e + 1)): at most 2^22 of them. (A row below 2^-100 counts as 0.)
-    const int e = (int)(__float_as_uint(most) >> 23) - 127;
+    // units of 2^(e - 22), most in [2^e, 2^(e + 1)) but for the binade's last part, which would have more of them than three signed digits
+    // (127 * 2^16 + 127 * 2^8 + 127): it counts as the next one's. (A row below 2^-100 counts as 0.)
+    const int e = (int)(__float_as_uint(__fmul_rn(most, 1.0041f)) >> 23) - 127;
     const bool none = odd || e < -100;
-    const float size = none ? 0.f : __uint_as_float((unsigned)(127 + 21 - e) << 23), per = negative ? -size : size;
-    q.unit = odd ? __builtin_nanf("") : none ? 0.f : __uint_as_float((unsigned)(127 - 21 + e) << 23);
+    const float size = none ? 0.f : __uint_as_float((unsigned)(127 + 22 - e) << 23), per = negative ? -size : size;
+    q.unit = odd ? __builtin_nanf("") : none ? 0.f : __uint_as_float((unsigned)(127 - 22 + e) << 23);
 #pragma unroll
     for (int c = 0; c < KC; ++c)
 #pragma unroll
@@ -171,7 +175,7 @@ struct RowView {
 // NP pages into a wave's 16 rows. key(page, tile) and value(page, tile): the lane's 16 bytes of a tile; keys_done and values_done: called
 // when the last of them is used. whole: every row sees all of them; behind: none of their
 // tokens is behind a row. Two pages at a time share the conversions of the second product's sums and the rescaling of o, a quarter of the vector
-// instructions of one: the weights go in as multiples of the pages' value scales, in units of 2^-22 of the largest such product.
+// instructions of one: the weights go in as multiples of the pages' value scales, in units of 1 / WEIGHT_UNITS of the largest such product.
 template <int KC, int EXTRA, int NP, typename Key, typename Value, typename KeysDone, typename ValuesDone>
 __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& q, const Key& key, const Value& value, const KeysDone& keys_done,
                                              const ValuesDone& values_done, const Pages<NP>& at, float factor, const Cap& cap, const RowView& row,
@@ -260,18 +264,18 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
     const float base = sees ? most : 0.f;
     // weights times value scales are at most `unit`
     float unit = 0.f, times[NP];
-    if constexpr (NP == 1) unit = at.v_scale[0], times[0] = 0x1p22f;
+    if constexpr (NP == 1) unit = at.v_scale[0], times[0] = WEIGHT_UNITS;
     else {
 #pragma unroll
         for (int p = 0; p < NP; ++p) unit = fmaxf(unit, __fmul_rn(fast_exp2(__fadd_rn(most_of[p], -base)), at.v_scale[p]));
         // (finite whatever the scales: a page that the row does not see may have one that is far larger)
-        const float per = unit > 0.f ? fminf(__fmul_rn(__builtin_amdgcn_rcpf(unit), 0x1p22f), 0x1p124f) : 0.f;
+        const float per = unit > 0.f ? fminf(__fmul_rn(__builtin_amdgcn_rcpf(unit), WEIGHT_UNITS), 0x1p124f) : 0.f;
 #pragma unroll
         for (int p = 0; p < NP; ++p) times[p] = fminf(__fmul_rn(at.v_scale[p], per), 0x1p126f);
     }
-    // The exact product less the rounded maximum can be above 0, by 2^-24 of it. Up to 2^22 the weights' three digits have room for that;
+    // The exact product less the rounded maximum can be above 0, by 2^-24 of it. Up to 2^12 the weights' three digits have room for that;
     // scores beyond are rounded first.
-    if (EXTRA == 0 && __any(__builtin_fabsf(base) > 0x1p22f)) {
+    if (EXTRA == 0 && __any(__builtin_fabsf(base) > 0x1p12f)) {
 #pragma unroll
         for (int p = 0; p < NP; ++p) {
 #pragma unroll
@@ -302,7 +306,7 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
     const float take = sees && (EXTRA != 2 || most != -__builtin_inff()) ? fast_exp2(__fadd_rn(most, -m)) : 0.f;
     s.m = m;
     s.l = __fmaf_rn(s.l, keep, __fmul_rn(sum, take));
-    const float put = __fmul_rn(__fmul_rn(take, 0x1p-22f), unit);
+    const float put = __fmul_rn(__fmul_rn(take, 1.f / WEIGHT_UNITS), unit);
     if (!__all(keep == 1.f)) {  // (a maximum seldom grows once a few pages are in)
 #pragma unroll
         for (int dt = 0; dt < 4 * KC; ++dt)
