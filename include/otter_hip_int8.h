@@ -636,8 +636,9 @@ typedef struct otter_hip_kv_batch {
 /* The batch's rows into the cache. keys, values: fp32, head_dim consecutive values for each head and the heads of a row one behind the
  * other; a row every key_stride / value_stride elements. A page's scale is s = max|x| / 127 over its tokens' finite values (0 below
  * 2^-100), code = x / s rounded half away from zero, exactly; NaN becomes 0, an infinity +-127. Where older tokens share the page, s is
- * no smaller than theirs was, and where it is larger their codes are rounded anew, code * s_old / s. A page that receives tokens must
- * not be named twice in the batch; full pages, and those only read, may be shared. */
+ * no smaller than theirs was, and where it is larger their codes are rounded anew, code * s_old / s. Rows are a sequence's last tokens:
+ * what an earlier call left behind them in their page is lost (a sequence may be cut and go on from there). A page that receives tokens
+ * must not be named twice in the batch; full pages, and those only read, may be shared. */
 int otter_hip_kv_append(const otter_hip_kv_cache* cache, const otter_hip_kv_batch* batch, const float* keys, size_t key_stride,
                         const float* values, size_t value_stride, void* stream);
 

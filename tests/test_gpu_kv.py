@@ -98,6 +98,18 @@ def test_append_rounds_older_tokens_anew(hip):
         s.check_read(s.batch(lengths, lengths))
 
 
+@pytest.mark.parametrize("dim", [64, 80])
+def test_sequences_cut_and_gone_on_from(hip, dim):
+    """Tokens taken back, as a draft that was not accepted: the next ones come where the first of them were."""
+    s = Setup(hip, np.random.default_rng(dim), 2, dim, [(100, 60), (64, 70), (3, 9), (0, 130)])
+    s.append(s.now, *s.normal(s.now, 2))
+    for kept, more in ([70, 64, 3, 129], [5, 1, 2, 1]), ([1, 64, 0, 63], [9, 66, 1, 2]):
+        b = s.batch(more, [n + m for n, m in zip(kept, more)])
+        s.append(b, *s.normal(b, 2))
+        s.check_read(s.batch([n + m for n, m in zip(kept, more)], [n + m for n, m in zip(kept, more)]))
+        s.check_attend(b, s.normal(b, 1, 4)[0])
+
+
 def test_append_of_ties_zeros_and_what_is_not_finite(hip):
     rng = np.random.default_rng(1)
     s = Setup(hip, rng, 2, 64, [(0, 70), (3, 40), (0, 5), (0, 64)])
@@ -331,6 +343,21 @@ def test_attend_of_queries_of_every_size(hip):
     big = np.ones_like(q)
     big[7:9] = q[7:9]
     s.check_attend(s.now, big, scale=1e-37)
+
+
+@pytest.mark.parametrize("dim", [64, 128, 192, 256])
+def test_queries_at_the_end_of_a_binade(hip, dim):
+    """The largest fixed-point numbers and sums there are: every element of a row the same, on either side of where the unit changes, and
+    every code of the keys 127 or -127; one row, and enough for the launch of many."""
+    for lengths in ([(130, 1)], [(0, 40), (70, 9)]):
+        s = Setup(hip, np.random.default_rng(dim), 1, dim, lengths)
+        k = np.where(np.arange(s.now[2])[:, None, None] % 2, -1, 1) * np.ones((1, 1, dim))
+        s.append(s.before, np.sign(s.normal(s.before, 1)[0][:, :, :1]) * np.ones((1, 1, dim), np.float32), s.normal(s.before, 1)[0])
+        s.append(s.now, k.astype(np.float32), s.normal(s.now, 1)[0])
+        sizes = np.float32([1, 1.9, 1.99182, 1.99183, 1.99184, 1.992, np.nextafter(np.float32(2), np.float32(0)), 2])
+        q = np.ones((s.now[2], 16, dim), np.float32) * np.concatenate([sizes, -sizes])[None, :, None]
+        s.check_attend(s.now, q, scale=1 / dim)
+        s.check_attend(s.now, q, scale=1 / dim, cap=3.0)
 
 
 def test_strides_between_rows(hip):
