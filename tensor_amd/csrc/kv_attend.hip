@@ -64,20 +64,17 @@ __device__ __forceinline__ float quad_sum(float x) {
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // times * tanh(x) / x for |x| < 1/2, of x * x; terms: TANH_TERM times that
-template <typename Terms>
-__device__ __forceinline__ float tanh_of_half(float y, const Terms& terms) {
-    float s = (float)terms[TANH_TERMS - 1];
+__device__ __forceinline__ float tanh_of_half(float y, const float (&terms)[TANH_TERMS]) {
+    float s = terms[TANH_TERMS - 1];
 #pragma unroll
-    for (int n = TANH_TERMS - 2; n >= 0; --n) s = __fmaf_rn(y, s, (float)terms[n]);
+    for (int n = TANH_TERMS - 2; n >= 0; --n) s = __fmaf_rn(y, s, terms[n]);
     return s;
 }
-// tanh. 1 - 2 / (exp(2 x) + 1) loses the bits of a small x, where the polynomial is taken. (The reciprocal is that of the hardware, off by
-// one unit in the last place at most: a division is ten instructions, a third of all here.)
-__device__ __forceinline__ float tanh_of(float x) {
-    const float a = __builtin_fabsf(x), y = __fmul_rn(x, x);
-    const float big = __fmaf_rn(-2.f, __builtin_amdgcn_rcpf(__fadd_rn(fast_exp2(__fmul_rn(a, 2.f * LOG2E)), 1.f)), 1.f);
-    const float small = __fmul_rn(a, tanh_of_half(y, TANH_TERM));
-    return __builtin_copysignf(a < 0.5f ? small : big, x);
+// tanh of |x| >= 1/2: 1 - 2 / (exp(2 |x|) + 1), which loses the bits of smaller ones. (The reciprocal is that of the hardware, off by one unit
+// in the last place at most: a division is ten instructions, a third of all here.)
+__device__ __forceinline__ float tanh_of_more(float x) {
+    const float e = fast_exp2(__fmul_rn(__builtin_fabsf(x), 2.f * LOG2E));
+    return __builtin_copysignf(__fmaf_rn(-2.f, __builtin_amdgcn_rcpf(__fadd_rn(e, 1.f)), 1.f), x);
 }
 
 // Three signed digits of four fixed-point numbers (u = number + 0x8080 in the low 24 bits): u's low two bytes less 128, and the third.
@@ -212,7 +209,8 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
             const auto scores = [&](const auto& last) {
                 float (&x)[4][4] = t[p];
                 if (EXTRA == 1 || cap.cap != 0.f) {
-                    // most scores are far below the cap: a third of the instructions for a page where all are below half of it
+                    // Most scores are far below the cap: a third of the instructions for a page where all are below half of it. The vote counts
+                    // slots that no row sees, whatever they hold: a score's bits are the same either way.
                     float far = 0.f;
 #pragma unroll
                     for (int i = 0; i < 16; ++i) far = fmaxf(far, __builtin_fabsf(x[i >> 2][i & 3]));
@@ -222,7 +220,11 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
                             x[i >> 2][i & 3] = last(i, x[i >> 2][i & 3], tanh_of_half(__fmul_rn(x[i >> 2][i & 3], x[i >> 2][i & 3]), cap.half));
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) x[i >> 2][i & 3] = last(i, tanh_of(x[i >> 2][i & 3]), cap.cap);
+                        for (int i = 0; i < 16; ++i) {
+                            const float y = x[i >> 2][i & 3], more = tanh_of_more(y), half = tanh_of_half(__fmul_rn(y, y), cap.half);
+                            const bool less = __builtin_fabsf(y) < 0.5f;
+                            x[i >> 2][i & 3] = last(i, less ? y : more, less ? half : cap.cap);
+                        }
                     }
                 } else {
 #pragma unroll
