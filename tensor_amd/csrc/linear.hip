@@ -259,8 +259,9 @@ __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
 }
 
 // The same launch with the rows' codes found by every workgroup for itself, in LDS, while its first weights are on their way: for the
-// row or two of a decoding step a launch in front of it takes as long as the product (one row of 2048 x 2048: 2.7 and 3.4 us). A row has W / (rows, rounded up to a power of two) waves, or a wave has several rows. 16-byte pieces of a row lie at their index
-// xor (row / 2) % 8, so that the 16 rows of an operand spread over the banks.
+// row or two of a decoding step a launch in front of it takes as long as the product (one row of 2048 x 2048: 2.7 and 3.4 us). A row has
+// W / (rows, rounded up to a power of two) waves, or a wave has several rows. 16-byte pieces of a row lie at their index xor (row / 2) % 8,
+// so that the 16 rows of an operand spread over the banks.
 template <int END, int W>
 __global__ void __launch_bounds__(64 * W) linear_rows_kernel(LinearArgs a, const float* __restrict__ x, size_t x_stride) {
     constexpr int G = END == LINEAR_GATED ? 2 : 1, AHEAD = 4;
@@ -509,6 +510,7 @@ static void launch_few(const LinearArgs& a, const LinearRows& r, hipStream_t str
 }
 
 constexpr int ROWS_W = 8;  // waves of linear_rows_kernel
+constexpr int ROWS_STATICS = 16 * ROWS_W * (int)sizeof(float);  // its rows' sizes, which lie in the same memory
 static int rows_lds(const LinearView& w, int rows) {
     const int codes = (rows < 16 ? rows : 16) * (int)linear_row_bytes(w.steps), sums = ROWS_W * (w.gated ? 2 : 1) * 1024;
     return codes > sums ? codes : sums;
@@ -535,7 +537,7 @@ static void launch_many(const LinearArgs& a, const LinearRows& r, hipStream_t st
 // the least traffic, 32 x 64 start the soonest. 4096 x 4096 weights with codes: 128 rows 22 us (few: 25), 512 rows 24.1 (64 x 64: 28.2),
 // 2048 rows 49.9 (32 x 64: 66.4), 8192 rows 163 (64 x 64: 192).
 int linear_choice(const LinearView& w, int rows) {
-    const bool fits = rows_lds(w, rows) <= 65536;
+    const bool fits = rows_lds(w, rows) + ROWS_STATICS <= 65536;  // (what a launch has without an attribute)
     if (w.force >= 0) return w.force == 4 && !fits ? 0 : w.force;
     // Codes within the launch: where a workgroup has few of them to find and the workgroups run beside each other. A row of 2048 x 2048 6.2 ->
     // 5.1 us, two of 4000 x 4096 8.6 -> 7.8, three 8.6 -> 11.5; a row of 1024 x 16000 6.3 -> 8.4 (one launch behind another without a pause;
