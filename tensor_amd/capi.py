@@ -707,15 +707,21 @@ class KvCache:
 
 
 class Linear:
-    """otter_hip_linear_t: int8 weights [experts, rows, in_features] (or [rows, in_features]: one expert) with a scale for each row."""
+    """otter_hip_linear_t: int8 weights [experts, rows, in_features] with a scale for each row, [experts, rows], and a bias likewise. One
+    expert may leave its axis out. Weights of another type are taken if every one is a whole number from -128 to 127."""
 
     def __init__(self, lib, *, weight, scale, bias=None, gated=False, act=0, act_p0=0.0):
         self.L = lib
         self.h = C.c_void_p()
-        w = np.ascontiguousarray(weight, np.int8)
+        given = np.asarray(weight)
+        with np.errstate(invalid="ignore"):  # (what no int8 stands for: refused below)
+            w = np.ascontiguousarray(given, np.int8)
+        if given.dtype != np.int8 and not np.array_equal(w, given):
+            raise HipError(-2, "linear: weights must be whole numbers from -128 to 127")
         w = w[None] if w.ndim == 2 else w
         s, b = (None if a is None else np.ascontiguousarray(a, np.float32) for a in (scale, bias))
-        if w.ndim != 3 or s.size != w.shape[0] * w.shape[1] or (b is not None and b.size != s.size) or (gated and w.shape[1] % 2):
+        shapes = (w.shape[:2], w.shape[1:2]) if len(w) == 1 else (w.shape[:2],)
+        if w.ndim != 3 or s.shape not in shapes or (b is not None and b.shape not in shapes) or (gated and w.shape[1] % 2):
             raise HipError(-2, "linear: weight [experts, rows, in_features], scale and bias [experts, rows]; an even number of rows with a gate")
         self.experts, rows, self.in_features = w.shape
         self.out_features = rows // 2 if gated else rows
