@@ -673,7 +673,7 @@ class KvBatch:
         lib.check_tensor(pages, i32, (n, None), "pages")
         if not 0 <= n_tokens < 2 ** 31 or pages.shape[1] >= 2 ** 31:
             raise HipError(-2, "kv_batch: n_tokens and max_pages have to be 0 or more, in 32 bits")
-        self.starts, self.lengths, self.pages, self.n_tokens = starts, lengths, pages, int(n_tokens)
+        self.L, self.starts, self.lengths, self.pages, self.n_tokens = lib, starts, lengths, pages, int(n_tokens)
         self.args = KvBatchArgs(n, self.n_tokens, pages.shape[1], starts.data_ptr(), lengths.data_ptr(), pages.data_ptr())
         self._bp = C.addressof(self.args)
 
@@ -692,18 +692,25 @@ class KvCache:
                                                                                     self.value_scales)])
         self._cp = C.addressof(self.args)  # the struct as the native call path takes it
 
+    def _batch(self, batch):
+        """The batch's struct; its arrays have to be on the cache's GPU."""
+        if batch.L.device_index != self.L.device_index:
+            raise HipError(-2, "kv_cache: the batch is on another GPU")
+        return batch._bp
+
     def append(self, batch, keys, values):
         """otter_hip_kv_append: keys and values [n_tokens, heads, head_dim], contiguous but for the stride between rows."""
-        self.L.native.kv_append(self._cp, batch._bp, keys, values, self.L.device_index)
+        self.L.native.kv_append(self._cp, self._batch(batch), keys, values, self.L.device_index)
 
     def read(self, batch, keys=None, values=None):
         """otter_hip_kv_read: the batch's rows as floats, [n_tokens, heads, head_dim] each. Returns (keys, values)."""
-        return self.L.native.kv_read(self._cp, batch._bp, keys, values, self.L.device_index)
+        return self.L.native.kv_read(self._cp, self._batch(batch), keys, values, self.L.device_index)
 
     def attend(self, batch, q, scale=None, cap=0.0, causal=True, window=0, slopes=None, out=None, workspace=None):
         """otter_hip_kv_attend: q [n_tokens, q_heads, head_dim], contiguous but for the stride between rows, over the cache.
         scale None: 1 / sqrt(head_dim). Returns out, of q's shape."""
-        return self.L.native.kv_attend(self._cp, batch._bp, q, scale, cap, causal, window, slopes, out, workspace, self.L.device_index)
+        return self.L.native.kv_attend(self._cp, self._batch(batch), q, scale, cap, causal, window, slopes, out, workspace,
+                                       self.L.device_index)
 
 
 class Linear:

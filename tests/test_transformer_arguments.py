@@ -50,3 +50,22 @@ def test_scales_and_biases_of_another_shape(shape):
 def test_one_expert_may_leave_its_axis_out(weight, shape):
     with pytest.raises(Reached):
         linear(weight, np.ones(shape, np.float32), np.ones(shape, np.float32))
+
+
+def test_batches_of_another_gpu():
+    """What a batch points to is memory of its library's GPU."""
+    class Gpu:
+        class native:
+            kv_append = kv_read = kv_attend = lambda *args: "called"
+
+        def __init__(self, device_index):
+            self.device_index = device_index
+
+    cache, batch = object.__new__(capi.KvCache), object.__new__(capi.KvBatch)
+    cache.L, cache._cp, batch._bp = Gpu(0), 0, 0
+    for call in (lambda: cache.append(batch, None, None), lambda: cache.read(batch), lambda: cache.attend(batch, None)):
+        batch.L = Gpu(1)
+        with pytest.raises(capi.HipError):
+            call()
+        batch.L = Gpu(0)
+        call()
