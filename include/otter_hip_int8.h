@@ -658,7 +658,7 @@ int otter_hip_kv_read(const otter_hip_kv_cache* cache, const otter_hip_kv_batch*
 typedef struct otter_hip_kv_attend_desc {
     int q_heads;
     float scale;
-    float cap;  /* 0: none */
+    float cap;  /* 0, or above 2^64: none */
     int causal;
     int window; /* 0: none */
     const float* slopes;

@@ -2375,6 +2375,10 @@ int otter_hip_kv_read(const otter_hip_kv_cache* cache, const otter_hip_kv_batch*
     return OTTER_HIP_OK;
 }
 
+// The cap that the launch takes. Above 2^64 it is none: what it would do to a score is below 2^-24 of it up to 2^52, and 1 / cap times a unit of a
+// score's fixed point would fall out of 32 bits. Below 2^-40 it is 2^-40: either leaves all weights the same, and the quotients are finite.
+static float kv_cap(float cap) { return cap > 0x1p64f ? 0.f : cap > 0.f ? std::max(cap, 0x1p-40f) : 0.f; }
+
 static int kv_attend_arguments(const char* who, const otter_hip_kv_cache* cache, const otter_hip_kv_batch* batch, const otter_hip_kv_attend_desc* d,
                                KvView* c, KvBatch* b, KvPlan* plan, size_t* bytes) {
     const std::string name(who);
@@ -2389,7 +2393,7 @@ static int kv_attend_arguments(const char* who, const otter_hip_kv_cache* cache,
     if ((size_t)b->n_tokens * d->q_heads >= (1ull << 31) || tiles * c->heads >= kMostGroups) return fail(OTTER_HIP_ERR_UNSUPPORTED, name + ": batch too large");
     *bytes = 0;
     if (b->n_seqs == 0 || b->n_tokens == 0) return OTTER_HIP_OK;
-    *plan = kv_attend_plan(b->n_tokens, b->n_seqs, (int)group, c->heads, c->chunks, d->cap != 0.f || d->slopes, b->max_pages);
+    *plan = kv_attend_plan(b->n_tokens, b->n_seqs, (int)group, c->heads, c->chunks, kv_cap(d->cap) != 0.f || d->slopes, b->max_pages);
     if (plan->splits > 1) {
         const size_t rows = (size_t)b->n_tokens * d->q_heads * plan->splits;
         *bytes = ((2 * rows + 3) / 4 * 4 + rows * c->dim) * sizeof(float);
@@ -2416,7 +2420,7 @@ int otter_hip_kv_attend(const otter_hip_kv_cache* cache, const otter_hip_kv_batc
     if (!q || !out) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_kv_attend: null");
     if (bytes && (!workspace || workspace_bytes < bytes)) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_kv_attend: workspace too small");
     if (bytes && ((size_t)workspace & 15)) return fail(OTTER_HIP_ERR_INVALID, "otter_hip_kv_attend: the workspace must be 16-byte aligned");
-    OHIP_CHECK(run_kv_attend(c, b, q, q_stride, out, desc->q_heads, desc->scale, desc->cap, desc->slopes, desc->causal, desc->window, plan,
+    OHIP_CHECK(run_kv_attend(c, b, q, q_stride, out, desc->q_heads, desc->scale, kv_cap(desc->cap), desc->slopes, desc->causal, desc->window, plan,
                              workspace, (hipStream_t)stream));
     return OTTER_HIP_OK;
 }
