@@ -652,8 +652,13 @@ int otter_hip_kv_read(const otter_hip_kv_cache* cache, const otter_hip_kv_batch*
  * of q that holds a NaN or an infinity gives NaN. Query head h reads key head h / (q_heads / heads).
  *   q    fp32, a row every q_stride elements, q_heads * head_dim consecutive values; out [n_tokens][q_heads][head_dim]
  *   slopes  device, [q_heads], or NULL; out overlaps neither q nor the workspace
- * The scores are those of q rounded to 23 bits below the row's largest element, all else is fp32. A row's result does not depend on the
- * rows of other sequences, but on how many workgroups its tokens are dealt to, which follows from n_seqs, n_tokens, max_pages and the heads.
+ * A row of q goes in rounded to multiples of 2^-22 of the power of two at or below its largest element (or of the next power, if that element is
+ * in the last half percent below it; a row below 2^-100 is 0), the weights exp(t_j - max) rounded to multiples of 2^-22.99 of the largest of
+ * their page or two pages, times the value scales; their products are summed exactly there, and all other arithmetic is fp32. A row that is so
+ * small that this rounding would show, as where the tokens with the weight have values near 0, takes the weights to 23, 46 or 69 bits more. So
+ * a row is off by about 2^-20 of itself, as with 32-bit sums; but one element of q that is far above the others takes bits from theirs.
+ * A row's bits do not depend on the rows of other sequences nor on what else is in the pages, but on how many workgroups its tokens are dealt to,
+ * which follows from n_seqs, n_tokens, max_pages and the heads.
  * workspace: otter_hip_kv_attend_workspace_bytes (0 where one workgroup has a row's tokens), 16-byte aligned. */
 typedef struct otter_hip_kv_attend_desc {
     int q_heads;

@@ -6,10 +6,11 @@
 // Both products run on the int8 matrix cores, on the cache's bytes as they are. The float operands go in as fixed point of three
 // 8-bit digits: a query row in units of 2^-22 of its largest element's binade, the weights exp(t_j - m) in units of 1 / WEIGHT_UNITS
 // of the largest weight that the row has in the page. Digit products and their sums are exact in 32 bits, so a score is off by what
-// rounding q to 23 bits makes of it, and a page's share of o by 2^-24 of the page's largest weight for each token: both are of the
-// size that sums in 32-bit floats have. (Half floats would need a second operand for the bits behind the 11th, and the bytes of
-// the cache converted for every row tile: two products at half the rate and five vector instructions for four bytes, against three
-// products at the full rate on bytes that are only loaded.)
+// rounding q to 23 bits makes of it, and a page's share of o by half a unit times the code for each token. Where o is large in these units,
+// that is what sums in 32-bit floats are off by. Where it is not -- the tokens that have the weight have values near 0, and o is what the
+// others make of theirs -- the digits behind follow (`finer` in the kernel). (Half floats would need a second operand for the bits behind
+// the 11th, and the bytes of the cache converted for every row tile: two products at half the rate and five vector instructions for four
+// bytes, against three products at the full rate on bytes that are only loaded.)
 //
 // A wave owns 16 query rows: the tokens of a sequence times the query heads that share a key head. The scores come transposed (keys x
 // rows), so a row's statistics and scale factors live in the lanes of its column, and the weights are already where the second
@@ -44,6 +45,11 @@ struct AttendArgs {
 
 // What a weight of 1 is as a whole number: a little below what three signed digits hold and, with the 0x8080 that makes them, below 2^23.
 constexpr float WEIGHT_UNITS = 8350000.f;
+
+// A row is made finer whose largest element is below this many units of its weights times a code of 1. The roundings, 0.29 units each, are 293
+// units together for 64 tokens with codes of 127: 2^-16.8 of that element, and 2^-18.6 with codes of normal values. Ordinary rows are ten times
+// above the limit: one token with the largest weight and a code of 40 is.
+constexpr float ROUGH = 0x1p25f;
 
 constexpr float LOG2E = 1.44269504088896340736f;
 
@@ -153,6 +159,22 @@ template <int KC>
 struct Running {
     float o[4 * KC][4];  // [16 dims][lane group's four]
     float m, l;          // maximum (log2), this lane's share of the sum
+    float second;        // the largest maximum of any step but the one that has m
+};
+// Of the steps that a wave takes, its rows together: the largest value scale (as an integer) and which of them raised the maximum of a row,
+// a bit each, the last for all from the 64th on. In scalar registers, as there is no vector register to spare; one vector instruction a step
+// for `second`.
+struct Steps {
+    unsigned scale;
+    unsigned long long raised;
+    int now;
+    __device__ float unit() const { return __fmul_rn(__uint_as_float(scale), 1.f / WEIGHT_UNITS); }  // what a unit of a weight is of o, at the most
+    __device__ bool raises(int step) const { return (raised >> min(step, 63)) & 1; }
+};
+// For REST of attend_pages: the lanes of which a unit is more than `least` of o get the digits behind the first three (level 1), six or nine.
+struct Finer {
+    float least;
+    int level;
 };
 
 // What a step of NP pages has beside their codes: the scales, and the positions of their first tokens.
@@ -173,10 +195,11 @@ struct RowView {
 // when the last of them is used. whole: every row sees all of them; behind: none of their
 // tokens is behind a row. Two pages at a time share the conversions of the second product's sums and the rescaling of o, a quarter of the vector
 // instructions of one: the weights go in as multiples of the pages' value scales, in units of 1 / WEIGHT_UNITS of the largest such product.
-template <int KC, int EXTRA, int NP, typename Key, typename Value, typename KeysDone, typename ValuesDone>
+// REST: the pages are in, and what the rounding of their weights has left out follows, three more digits.
+template <int KC, int EXTRA, int NP, bool REST, typename Key, typename Value, typename KeysDone, typename ValuesDone>
 __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& q, const Key& key, const Value& value, const KeysDone& keys_done,
                                              const ValuesDone& values_done, const Pages<NP>& at, float factor, const Cap& cap, const RowView& row,
-                                             bool whole, bool behind) {
+                                             bool whole, bool behind, Steps& steps, const Finer& finer = {}) {
     const int g = (int)(threadIdx.x >> 4) & 3;
     // scores (log2) are t * unit_of + away; without cap and slopes the product is left to the subtraction of the maximum
     float t[NP][4][4], most_of[NP], unit_of[NP], away = 0.f;
@@ -285,6 +308,13 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
             unit_of[p] = 1.f;
         }
     }
+    float rest = 0.f;
+    if constexpr (REST) {
+        const float share = fast_exp2(__fadd_rn(EXTRA == 2 && KC == 1 ? __fadd_rn(most, away) : most, -s.m));
+        const float put = __fmul_rn(__fmul_rn(share, 1.f / WEIGHT_UNITS), unit);
+        rest = sees && put > finer.least ? put : 0.f;
+        if (!__any(rest > 0.f)) return;
+    }
     float sum = 0.f;
     v4i w[NP][3];
 #pragma unroll
@@ -295,21 +325,48 @@ __device__ __forceinline__ void attend_pages(Running<KC>& s, const Queries<KC>& 
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const float e = fast_exp2(__fmaf_rn(t[p][kt][r], unit_of[p], -base));
-                sum = __fadd_rn(sum, e);
-                u[r] = __float_as_uint(__fmaf_rn(e, times[p], 8388608.f + 32896.f));  // 2^23 + 0x8080: the mantissa is the rounded number
+                const float number = __fmaf_rn(e, times[p], 8388608.f + 32896.f);  // 2^23 + 0x8080: the mantissa is the rounded number
+                if constexpr (!REST) {
+                    sum = __fadd_rn(sum, e);
+                    u[r] = __float_as_uint(number);
+                } else {  // (the differences are exact, or to 24 bits of the weight itself)
+                    float left = __fmul_rn(__fmaf_rn(e, times[p], -__fadd_rn(number, -(8388608.f + 32896.f))), 0x1p23f);
+                    for (int n = 1; n < finer.level; ++n) left = __fmul_rn(__fadd_rn(left, -__builtin_rintf(left)), 0x1p23f);
+                    u[r] = (unsigned)((int)__builtin_rintf(left) + 0x8080);
+                }
             }
             int low, mid, high;
             split_digits(u, low, mid, high);
             w[p][2][kt] = low, w[p][1][kt] = mid, w[p][0][kt] = high;
         }
     if constexpr (EXTRA == 2 && KC == 1) most = __fadd_rn(most, away);
+    if constexpr (REST) {
+        const float per = __uint_as_float((unsigned)(127 - 23 * finer.level) << 23);
+#pragma unroll
+        for (int dt = 0; dt < 4 * KC; ++dt) {
+            v4i a[3] = {};
+#pragma unroll
+            for (int p = 0; p < NP; ++p) {
+                const v4i v = value(p, dt);
+#pragma unroll
+                for (int n = 0; n < 3; ++n) a[n] = mma(v, w[p][n], a[n]);
+            }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s.o[dt][r] = __fmaf_rn(__fmul_rn(join_digits(a[0][r], a[1][r], a[2][r]), per), rest, s.o[dt][r]);
+        }
+        return;
+    }
     const float m = fmaxf(s.m, most);
     const float keep = s.m == -__builtin_inff() ? 0.f : fast_exp2(__fadd_rn(s.m, -m));
     const float take = sees && (EXTRA != 2 || most != -__builtin_inff()) ? fast_exp2(__fadd_rn(most, -m)) : 0.f;
+    s.second = __builtin_amdgcn_fmed3f(s.second, s.m, most);
     s.m = m;
     s.l = __fmaf_rn(s.l, keep, __fmul_rn(sum, take));
     const float put = __fmul_rn(__fmul_rn(take, 1.f / WEIGHT_UNITS), unit);
+#pragma unroll
+    for (int p = 0; p < NP; ++p) steps.scale = max(steps.scale, __float_as_uint(at.v_scale[p]));
     if (!__all(keep == 1.f)) {  // (a maximum seldom grows once a few pages are in)
+        steps.raised |= 1ull << min(steps.now, 63);
 #pragma unroll
         for (int dt = 0; dt < 4 * KC; ++dt)
 #pragma unroll
@@ -369,9 +426,11 @@ constexpr int kv_lds_bytes(bool staged, int waves) {
 // what they have in LDS. A wave's next page is on its way into registers while it works on one. With STAGED and more than 32 rows the
 // four waves read their pages, which are the same, from LDS, two at a time (see attend_pages), the next two on their way into registers: the
 // faster way only where it leaves room for three workgroups a compute unit and there are as many, by 6 % for 65 to 128 dims (4096 rows on 14
-// thousand tokens: 1.33 ms, 1.45 without, and 1.46 with two buffers in LDS and two workgroups).
+// thousand tokens: 1.33 ms, 1.45 without, and 1.46 with two buffers in LDS and two workgroups). Without cap and slopes up to 64 dims leave
+// room for four waves a SIMD if the compiler is told so (128 registers, else 130).
 template <int KC, int EXTRA, bool STAGED, int WAVES>
-__global__ void __launch_bounds__(64 * WAVES, STAGED ? 3 : EXTRA < 2 ? 1 : KC == 1 ? 3 : KC <= 3 ? 2 : 1) kv_attend_kernel(AttendArgs a) {
+__global__ void __launch_bounds__(64 * WAVES, STAGED ? 3 : KC == 1 && EXTRA == 0 ? 4 : EXTRA < 2 ? 1 : KC == 1 ? 3 : KC <= 3 ? 2 : 1)
+    kv_attend_kernel(AttendArgs a) {
     static_assert(!STAGED || WAVES == 4, "the staging is dealt to four waves");
     __shared__ __attribute__((aligned(16))) unsigned char lds[kv_lds_bytes<KC>(STAGED, WAVES)];
     typedef float JoinedRows[16][64 * KC + 4];
@@ -418,7 +477,7 @@ __global__ void __launch_bounds__(64 * WAVES, STAGED ? 3 : EXTRA < 2 ? 1 : KC ==
     const int first_lo = __builtin_amdgcn_readlane(view.lo, 0), last_lo = __builtin_amdgcn_readlane(view.lo, 15);
 
     Running<KC> run;
-    run.m = -__builtin_inff(), run.l = 0.f;
+    run.m = -__builtin_inff(), run.l = 0.f, run.second = -__builtin_inff();
 #pragma unroll
     for (int dt = 0; dt < 4 * KC; ++dt)
 #pragma unroll
@@ -438,6 +497,42 @@ __global__ void __launch_bounds__(64 * WAVES, STAGED ? 3 : EXTRA < 2 ? 1 : KC ==
         factor = __fmul_rn(q.unit, __builtin_fabsf(a.scale));
     };
     const auto nothing = [] {};
+    // Steps of NP pages, as they were taken, once more for the rows of which the rounding of the weights has left too little: whose largest element
+    // is below ROUGH of the units, those of the step with the maximum and the root of the others' squares at the most. Mostly the first is what is
+    // large, and only steps that raised a maximum are gone through; with the others too if they alone may be too much. At the end of the walk, since
+    // only then is it known what o is: an ordinary row pays 20 to 40 instructions (the launch for one token on 520 takes 0.15 us more).
+    Steps steps = {0, 0, 0};
+    const auto finer = [&](auto pages) {
+        constexpr int NP = decltype(pages)::value;
+        const float many = __builtin_amdgcn_sqrtf((float)((walk.to - walk.from + NP - 1) / NP));
+        const float others = __fmul_rn(__fmul_rn(fast_exp2(__fadd_rn(run.second, -run.m)), steps.unit()), many);
+        float rough = ROUGH;
+#pragma unroll 1
+        for (int level = 1; level <= 3; ++level, rough *= 0x1p-23f) {
+            float size = 0.f;
+#pragma unroll
+            for (int dt = 0; dt < 4 * KC; ++dt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) size = fmaxf(size, __builtin_fabsf(run.o[dt][e]));
+            size = quad_max(size);
+            const bool some = run.m != -__builtin_inff() && size < __fmul_rn(__fadd_rn(steps.unit(), others), rough);
+            const bool all = size < __fmul_rn(others, rough);
+            if (__builtin_expect(!__any(some), 1)) return;
+            const Finer now = {some ? __fdiv_rn(size, __fmul_rn(many, rough)) : __builtin_inff(), level};
+#pragma unroll 1
+            for (int pg = walk.from, step = 0; pg < walk.to; pg += NP, ++step) {
+                if (!steps.raises(step) && !__any(all)) continue;
+                PageWalk one = {walk.table, pg, min(pg + NP, walk.to), 0};
+                const int8_t *kp[NP], *vp[NP];
+                const Pages<NP> at = pages_at<NP>(a.c, head, one, pg, kp, vp);
+                const auto from = [&](const int8_t* page, int tile) { return *reinterpret_cast<const v4i*>(page + tile * 1024 + lane16); };
+                attend_pages<KC, EXTRA, NP, true>(
+                    run, q, [&](int n, int tile) { return from(kp[n], tile); }, [&](int n, int tile) { return from(vp[n], tile); }, nothing, nothing,
+                    at, factor, cap, view, at.all && (pg + NP) * KV_BLOCK <= first_hi && pg * KV_BLOCK >= last_lo,
+                    NP == 1 && (pg + 1) * KV_BLOCK <= first_p + 1, steps, now);
+            }
+        }
+    };
     if (STAGED && shares == 1) {
         if constexpr (STAGED) {
             constexpr int NP = 2, TILES = NP * 8 * KC, MINE = TILES / 4;
@@ -472,12 +567,15 @@ __global__ void __launch_bounds__(64 * WAVES, STAGED ? 3 : EXTRA < 2 ? 1 : KC ==
                     if (works && pg * KV_BLOCK < last_hi && (pg + NP) * KV_BLOCK > first_lo) {
                         const bool whole = at.all && (pg + NP) * KV_BLOCK <= first_hi && pg * KV_BLOCK >= last_lo;
                         const v4i* const from = buffer + lane;
-                        attend_pages<KC, EXTRA, NP>(
+                        steps.now = (pg - walk.from) / NP;
+                        attend_pages<KC, EXTRA, NP, false>(
                             run, q, [&](int n, int tile) { return from[(n * 8 * KC + tile) * 64]; },
-                            [&](int n, int tile) { return from[(n * 8 * KC + 4 * KC + tile) * 64]; }, nothing, nothing, at, factor, cap, view, whole, false);
+                            [&](int n, int tile) { return from[(n * 8 * KC + 4 * KC + tile) * 64]; }, nothing, nothing, at, factor, cap, view, whole,
+                            false, steps);
                     }
                     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");  // nobody reads them any more
                 }
+                finer(std::integral_constant<int, NP>{});
             }
         }
     } else if (works) {
@@ -496,9 +594,10 @@ __global__ void __launch_bounds__(64 * WAVES, STAGED ? 3 : EXTRA < 2 ? 1 : KC ==
             load(values, vp[0]);
             const auto page = [&](int pg, const auto& keys_done, const auto& values_done) {
                 const bool whole = at.all && (pg + 1) * KV_BLOCK <= first_hi && pg * KV_BLOCK >= last_lo;
-                attend_pages<KC, EXTRA, 1>(
+                steps.now = pg - walk.from;
+                attend_pages<KC, EXTRA, 1, false>(
                     run, q, [&](int, int tile) { return keys[tile]; }, [&](int, int tile) { return values[tile]; }, keys_done, values_done, at, factor,
-                    cap, view, whole, (pg + 1) * KV_BLOCK <= first_p + 1);
+                    cap, view, whole, (pg + 1) * KV_BLOCK <= first_p + 1, steps);
             };
             int pg = walk.from;
             for (; pg + 1 < walk.to; ++pg) {
@@ -507,6 +606,7 @@ __global__ void __launch_bounds__(64 * WAVES, STAGED ? 3 : EXTRA < 2 ? 1 : KC ==
                 at = next;
             }
             page(pg, nothing, nothing);
+            finer(std::integral_constant<int, 1>{});
         }
     }
     run.l = quad_sum(run.l);
