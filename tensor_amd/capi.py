@@ -733,8 +733,9 @@ class Linear:
         self.experts, rows, self.in_features = w.shape
         self.out_features = rows // 2 if gated else rows
         d = LinearDesc(self.experts, self.in_features, self.out_features, int(gated), act, act_p0)
-        lib._check(lib.lib.otter_hip_linear_create(C.byref(d), w.ctypes.data_as(C.c_void_p), s.ctypes.data_as(C.c_void_p),
-                                                   b.ctypes.data_as(C.c_void_p) if b is not None else None, C.byref(self.h)))
+        with lib.torch.cuda.device(lib.device_index):  # (the weights go to the current GPU)
+            lib._check(lib.lib.otter_hip_linear_create(C.byref(d), w.ctypes.data_as(C.c_void_p), s.ctypes.data_as(C.c_void_p),
+                                                       b.ctypes.data_as(C.c_void_p) if b is not None else None, C.byref(self.h)))
         self._hp = self.h.value  # the handle as the native call path takes it
 
     def kernel_kind(self, rows):

@@ -69,3 +69,34 @@ def test_batches_of_another_gpu():
             call()
         batch.L = Gpu(0)
         call()
+
+
+def test_a_layer_is_made_on_its_librarys_gpu():
+    """Whatever GPU is the current one."""
+    from contextlib import contextmanager
+    current = [0]
+
+    class Gpu(NoGpu):
+        device_index = 1
+
+        class torch:
+            class cuda:
+                @staticmethod
+                @contextmanager
+                def device(index):
+                    current.append(index)
+                    yield
+                    current.pop()
+
+        class lib:
+            @staticmethod
+            def otter_hip_linear_create(*args):
+                made_on.append(current[-1])
+                return 0
+
+        def _check(self, rc):
+            assert rc == 0
+
+    made_on = []
+    capi.Linear(Gpu(), weight=ONES, scale=np.ones((2, 4), np.float32))
+    assert made_on == [1] and current == [0]
