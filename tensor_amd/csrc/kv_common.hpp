@@ -144,7 +144,7 @@ __device__ __forceinline__ int code_of(float x, float s, float inv) {
 // The four codes of a word, and whether one of them may be wrong: then code_of has to find them. c = rint(x / s), the quotient off by
 // less than 2^-15, is right where |x - c s| < s / 2; one fused multiply-add has that difference, rounded, and a rounding does not pass s / 2.
 // (Not below s / 2: the middle between two codes, a code that is off by one, an infinity, NaN.) Eight instructions a code with their
-// packing, where code_of is twenty: one token for each of 48 sequences appended in 5.6 us for 6.9, 8192 rows of 2816 rounded in 13.0 for 15.0.
+// packing, where code_of is twenty: one token for each of 48 sequences appended in 5.6 us for 6.9, 4096 rows of 2816 rounded in 13.0 for 15.0.
 struct Coder {
     float s, inv, half;
     __device__ explicit Coder(float scale) : s(scale) {

@@ -211,8 +211,7 @@ __device__ __forceinline__ bool linear_quads(const LinearArgs& a) { return a.w.o
 
 // 16 outputs (gated: 16 of either half) x 16 rows a workgroup, the inputs dealt to its W waves, whose sums meet in LDS. Both operands
 // come straight from memory in lane order, several steps of them asked for before the first is used; this is the launch for few rows,
-// where reading the weights is the work. (32 and 64 rows a workgroup, which read the weights less often, were the fastest of all launches
-// for no size.)
+// where reading the weights is the work. It reads them once for every 16 rows: 64 rows of 4096 x 4096 take 15.9 us with their codes, 32 11.0.
 template <int END, int W>
 __global__ void __launch_bounds__(64 * W) linear_few_kernel(LinearArgs a) {
     constexpr int G = END == LINEAR_GATED ? 2 : 1, AHEAD = 4;
@@ -530,12 +529,13 @@ static void launch_many(const LinearArgs& a, const LinearRows& r, hipStream_t st
 #undef CALL
 }
 
-// The launch that is the fastest by a model fitted to 92 measured products (16 to 128 steps of inputs, 512 to 8192 outputs, 1 to 16384
-// rows, 1 to 64 experts; microseconds without the codes): 1 % over the fastest of the four on the mean, 18 % at most. The one for few rows
-// reads weights and rows from the caches at 8 TB/s, 16 x 16 results at a time, but waits 1.2 for every 32 steps. The others take `each`
-// for a stage of a workgroup by itself and `busy` where every compute unit has one, n times that for n: 64 x 128 results a wave are
-// the least traffic, 32 x 64 start the soonest. 4096 x 4096 weights with codes: 128 rows 22 us (few: 25), 512 rows 24.1 (64 x 64: 28.2),
-// 2048 rows 49.9 (32 x 64: 66.4), 8192 rows 163 (64 x 64: 192).
+// The launch that is the fastest by a model of microseconds without the codes, fitted to measured products of 16 to 128 steps of inputs, 512 to
+// 8192 outputs, 1 to 16384 rows and 1 to 64 experts. Over 92 such products (profiles/linear_launch_choice.md) the choice is 1.1 % over the
+// fastest of the five launches on the mean and 25 % at most, where 16 rows go to 64 experts. The one for few rows reads weights and rows from
+// the caches at 8 TB/s, 16 x 16 results at a time, but waits 1.2 for every 32 steps. The others take `each` for a stage of a workgroup by itself
+// and `busy` where every compute unit has one, n times that for n: 64 x 128 results a wave are the least traffic, 32 x 64 start the soonest.
+// 4096 x 4096 weights with codes: 128 rows 20.6 us (few: 25.9), 512 rows 25.4 (64 x 64: 29.7), 4096 rows 86 (32 x 64: 124), 16384 rows 350
+// (64 x 64: 430).
 int linear_choice(const LinearView& w, int rows) {
     const bool fits = rows_lds(w, rows) + ROWS_STATICS <= 65536;  // (what a launch has without an attribute)
     if (w.force >= 0) return w.force == 4 && !fits ? 0 : w.force;
