@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(64 * WAVES, STAGED ? 3 : KC == 1 && EXTRA == 0
     // Steps of NP pages, as they were taken, once more for the rows of which the rounding of the weights has left too little: whose largest element
     // is below ROUGH of the units, those of the step with the maximum and the root of the others' squares at the most. Mostly the first is what is
     // large, and only steps that raised a maximum are gone through; with the others too if they alone may be too much. At the end of the walk, since
-    // only then is it known what o is: an ordinary row pays 20 to 40 instructions (the launch for one token on 520 takes 0.2 us more), and batches
+    // only then is it known what o is: an ordinary row pays 20 to 40 instructions (the launch for one token on 520 takes 0.3 us more), and batches
     // whose rows all have such a token at their front 3 to 6 % (4096 rows on 14 thousand tokens: 1.35 -> 1.43 ms).
     Steps steps = {0, 0, 0};
     const auto finer = [&](auto pages) {
