@@ -656,7 +656,8 @@ int otter_hip_kv_read(const otter_hip_kv_cache* cache, const otter_hip_kv_batch*
  * in the last half percent below it; a row below 2^-100 is 0), the weights exp(t_j - max) rounded to multiples of 2^-22.99 of the largest of
  * their page or two pages, times the value scales; their products are summed exactly there, and all other arithmetic is fp32. A row that is so
  * small that this rounding would show, as where the tokens with the weight have values near 0, takes the weights to 23, 46 or 69 bits more. So
- * a row is off by about 2^-20 of itself, as with 32-bit sums; but one element of q that is far above the others takes bits from theirs.
+ * a row is off by about 2^-20 of itself, as with 32-bit sums, and by 2^-16.5 where scores around 25 meet values near 0; but one element of q that
+ * is far above the others takes bits from theirs.
  * A row's bits do not depend on the rows of other sequences nor on what else is in the pages, but on how many workgroups its tokens are dealt to,
  * which follows from n_seqs, n_tokens, max_pages and the heads.
  * workspace: otter_hip_kv_attend_workspace_bytes (0 where one workgroup has a row's tokens), 16-byte aligned. */
