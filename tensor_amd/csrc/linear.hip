@@ -530,7 +530,7 @@ static void launch_many(const LinearArgs& a, const LinearRows& r, hipStream_t st
 }
 
 // The launch that is the fastest by a model of microseconds without the codes, fitted to measured products of 16 to 128 steps of inputs, 512 to
-// 8192 outputs, 1 to 16384 rows and 1 to 64 experts. Over 92 such products (profiles/linear_launch_choice.md) the choice is 1.1 % over the
+// 8192 outputs, 1 to 16384 rows and 1 to 64 experts. Over 92 such products, whose times profiles/ holds, the choice is 1.1 % over the
 // fastest of the five launches on the mean and 25 % at most, where 16 rows go to 64 experts. The one for few rows reads weights and rows from
 // the caches at 8 TB/s, 16 x 16 results at a time, but waits 1.2 for every 32 steps. The others take `each` for a stage of a workgroup by itself
 // and `busy` where every compute unit has one, n times that for n: 64 x 128 results a wave are the least traffic, 32 x 64 start the soonest.
